@@ -34,11 +34,11 @@ def build_cpp(verbose=False, jobs=None):
     _run(["cmake", "--build", BUILD_DIR, "-j", str(jobs)], verbose)
 
 
-def build_hip(verbose=False):
-    """gfx950 GPU probe library (devspace_amd/ops/gpuprobe.hip)."""
+def build_hip(verbose=False, force=False):
+    """gfx950 GPU probe library and fused-ops extension (devspace_amd/ops)."""
     from devspace_amd.ops import build as ops_build
 
-    return ops_build.build(verbose=verbose)
+    return ops_build.build(verbose=verbose, force=force)
 
 
 def write_example_kit(verbose=False):
@@ -52,10 +52,10 @@ def write_example_kit(verbose=False):
         print("+ workload kit -> examples/rocm-pytorch/devspace_amd: " + ", ".join(written), flush=True)
 
 
-def build_all(verbose=False):
+def build_all(verbose=False, force_hip=False):
     build_cpp(verbose=verbose)
     try:
-        build_hip(verbose=verbose)
+        build_hip(verbose=verbose, force=force_hip)
     except FileNotFoundError as e:  # hipcc missing: CPU-only environments still get the tool
         print(f"skipping HIP build: {e}", flush=True)
     write_example_kit(verbose=verbose)

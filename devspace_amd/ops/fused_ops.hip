@@ -1553,15 +1553,13 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& tgt, int64_
 
 }  // namespace
 
-// SHA-256 of this file, passed by devspace_amd/ops/build.py: the loader checks the extension it
-// imports was built from the source next to it (no stale kernels after an edit or a checkout)
-#ifndef DEVSPACE_SOURCE_SHA
-#define DEVSPACE_SOURCE_SHA "unknown"
-#endif
+// SHA-256 of the sources, linked in by devspace_amd/ops/build.py: the loader checks the extension it
+// imports was built from the sources next to it (no stale kernels after an edit or a checkout)
+extern const char devspace_source_sha[];
 
 PYBIND11_MODULE(_fused_ops, m) {
   m.doc() = "gfx950 fused training ops (RMSNorm, SwiGLU, cross-entropy)";
-  m.attr("source_sha") = DEVSPACE_SOURCE_SHA;
+  m.attr("source_sha") = pybind11::str(devspace_source_sha);
   m.def("rmsnorm_supported", &rmsnorm_supported);
   // differentiable entry points (C++ autograd)
   m.def("rms_norm", &rms_norm);

@@ -5,6 +5,7 @@
     x, h = fused.add_rms_norm(x, delta, norm.weight)  # x += delta; h = norm(x), one kernel
     y = fused.swiglu(h)                   # silu(h[..., :H]) * h[..., H:]
     loss = fused.cross_entropy(logits, t) # mean CE on bf16 logits [N, V]
+    qkv = fused.rotary_qkv(qkv, positions, freqs)     # q and k turned by their positions
 
 On a GPU the HIP kernels are mandatory: if the in-tree extension is missing or broken the
 first call raises (no silent eager fallback). On CPU tensors (tests, CPU smoke runs) the plain
@@ -12,6 +13,8 @@ PyTorch formulation is used.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn as nn
@@ -178,6 +181,138 @@ def attention(qkv: torch.Tensor, causal: bool = True, scale: float | None = None
     o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=causal,
                                        scale=scale)
     return o.transpose(1, 2)
+
+
+# ------------------------------------------------------------------------------ rotary positions
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       original_length: int = 4096, fast: float = 32.0, slow: float = 1.0, device=None):
+    """(freqs, magnitude) for rotary positions on the first `dim` columns of a head: freqs is a float64
+    tensor of dim / 2 angles per position, base^(-2i/dim), scaled for contexts `factor` times as long:
+
+      "linear"  every frequency divided by the factor (positions squeezed)
+      "ntk"     the base raised to base * factor^(dim / (dim - 2)): the fastest pair keeps its
+                frequency, the slowest is divided by the factor
+      "yarn"    pairs that turn at least `fast` times within `original_length` keep their frequency,
+                those that turn at most `slow` times are divided by the factor, a ramp between them;
+                q and k are multiplied by the magnitude 0.1 ln(factor) + 1
+    """
+    if dim < 2 or dim % 2:
+        raise ValueError("rotary_frequencies: dim must be even and at least 2")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r}")
+    if base <= 0 or factor < 1 or original_length < 1 or fast <= slow:
+        raise ValueError("rotary_frequencies: base > 0, factor >= 1, original_length >= 1 and fast > slow wanted")
+    if scaling == "ntk" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    freqs = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    magnitude = 1.0
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "yarn":
+        turns = original_length * freqs / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        freqs = freqs * keep + freqs / factor * (1 - keep)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    return freqs.to(device), magnitude
+
+
+def _check_rotary(x, dims, freqs):
+    if x.dim() != dims:
+        raise ValueError("rotary: heads must be [B, T, H, D]" if dims == 4 else "rotary: qkv must be [B, T, 3, H, D]")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not 1 <= freqs.numel() <= x.shape[-1] // 2:
+        raise ValueError("rotary: freqs must be a 1-D float64 tensor of 1 to head_dim / 2 values")
+
+
+def _rotary_eager(x, positions, freqs, interleaved, magnitude):
+    """The formula in PyTorch ops (x [B, T, H, D]): angles in 64 bits, the turn in 32 (64 for float64)."""
+    b, t, _, d = x.shape
+    if not isinstance(positions, torch.Tensor):
+        positions = torch.arange(t, device=x.device) + int(positions or 0)
+    if positions.shape not in ((t,), (1, t), (b, t)) or positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError("rotary: positions must be int64 or int32 and [T], [1, T] or [B, T]")
+    angle = (positions.double()[..., None] * freqs)[..., None, :]
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    cos, sin = (angle.cos() * magnitude).to(wide), (angle.sin() * magnitude).to(wide)
+    n = freqs.numel()
+    y = x.to(wide)
+    u, v = (y[..., 0:2 * n:2], y[..., 1:2 * n:2]) if interleaved else (y[..., :n], y[..., n:2 * n])
+    turned = (u * cos - v * sin, u * sin + v * cos)
+    turned = torch.stack(turned, -1).flatten(-2) if interleaved else torch.cat(turned, -1)
+    return torch.cat((turned, y[..., 2 * n:]), -1).to(x.dtype)
+
+
+_HIP_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _rotary_hip(x, k, packed, positions, freqs, interleaved, magnitude):
+    pos = positions if isinstance(positions, torch.Tensor) else None
+    return ext().rotary(x, k, packed, pos, 0 if pos is not None else int(positions or 0), freqs, bool(interleaved),
+                        float(magnitude))
+
+
+def rotary(x: torch.Tensor, positions, freqs: torch.Tensor, interleaved: bool = False,
+           magnitude: float = 1.0) -> torch.Tensor:
+    """Rotary positions on heads x [B, T, H, D] (any strides): pair i of the first 2 * len(freqs) columns
+    is turned by position * freqs[i] and multiplied by `magnitude`; the other columns are carried over.
+
+    positions: an int64 or int32 tensor [T], [1, T] or [B, T], or a whole number: the position of
+    token 0 (None: 0). interleaved: pairs are neighbouring columns (2i, 2i + 1) instead of
+    (i, i + len(freqs)). Gradients flow to x. bfloat16, float16 and float32 run the gfx950 kernel on a GPU."""
+    _check_rotary(x, 4, freqs)
+    if x.is_cuda and x.dtype in _HIP_FLOATS:
+        return _rotary_hip(x, None, False, positions, freqs, interleaved, magnitude)[0]
+    return _rotary_eager(x, positions, freqs, interleaved, magnitude)
+
+
+def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions, freqs: torch.Tensor, interleaved: bool = False,
+              magnitude: float = 1.0):
+    """rotary() of queries [B, T, H, D] and keys [B, T, N, D] in one launch: (q', k')."""
+    _check_rotary(q, 4, freqs)
+    _check_rotary(k, 4, freqs)
+    if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.dtype != k.dtype or q.device != k.device:
+        raise ValueError("rotary: q and k must agree in B, T, D, type and device")
+    if q.is_cuda and q.dtype in _HIP_FLOATS:
+        return tuple(_rotary_hip(q, k, False, positions, freqs, interleaved, magnitude))
+    return tuple(_rotary_eager(x, positions, freqs, interleaved, magnitude) for x in (q, k))
+
+
+def rotary_qkv(qkv: torch.Tensor, positions, freqs: torch.Tensor, interleaved: bool = False,
+               magnitude: float = 1.0) -> torch.Tensor:
+    """rotary() of the q and k of a packed projection [B, T, 3, H, D], v carried over: what attention()
+    reads, in one launch."""
+    _check_rotary(qkv, 5, freqs)
+    if qkv.shape[2] != 3:
+        raise ValueError("rotary: qkv must be [B, T, 3, H, D]")
+    if qkv.is_cuda and qkv.dtype in _HIP_FLOATS:
+        return _rotary_hip(qkv, None, True, positions, freqs, interleaved, magnitude)[0]
+    q, k, v = qkv.unbind(2)
+    return torch.stack([_rotary_eager(x, positions, freqs, interleaved, magnitude) for x in (q, k)] + [v], 2)
+
+
+class Rotary(nn.Module):
+    """Rotary positions of a model: keeps the frequencies (a buffer that stays float64 when the module is
+    cast) and applies them to a packed qkv or to q and k."""
+
+    def __init__(self, dim: int, interleaved: bool = False, base: float = 10000.0, scaling: str = "none",
+                 factor: float = 1.0, original_length: int = 4096):
+        super().__init__()
+        self.interleaved = interleaved
+        freqs, self.magnitude = rotary_frequencies(dim, base, scaling, factor, original_length)
+        self.register_buffer("freqs", freqs, persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        exact = self.freqs
+        super()._apply(fn, recurse)
+        if self.freqs.dtype != torch.float64:  # .bfloat16() and the like: move, but keep the exact values
+            self.freqs = exact.to(self.freqs.device)
+        return self
+
+    def forward(self, q, k=None, positions=None):
+        if k is None:
+            return rotary_qkv(q, positions, self.freqs, self.interleaved, self.magnitude)
+        return rotary_qk(q, k, positions, self.freqs, self.interleaved, self.magnitude)
 
 
 # ------------------------------------------------------------------------------ AdamW

@@ -17,38 +17,19 @@
 //
 // Reference parity: this is workload-side code (the tool itself has no
 // numeric path); numerics are tested against fp32 PyTorch in tests/test_fused_ops.py.
-#include <hip/hip_runtime.h>
-#include <torch/extension.h>
+#include "fused_common.h"
+
 #include <ATen/Parallel.h>
 
 #include <atomic>
 #include <thread>
 #include <vector>
-#include <c10/hip/HIPStream.h>
 
-#include <cmath>
-#include <cstdint>
+void register_rotary(pybind11::module_& m);
 
 namespace {
 
-typedef unsigned short u16;
-template <int N>
-using u16v = u16 __attribute__((ext_vector_type(N)));
-typedef u16v<8> u16x8;
-
 constexpr int kBlock = 256;  // 4 waves
-
-__device__ __forceinline__ float b2f(u16 v) { return __uint_as_float((unsigned)v << 16); }
-__device__ __forceinline__ u16 f2b(float f) {
-  __bf16 b = (__bf16)f;  // v_cvt_pk_bf16_f32: RNE, NaN stays NaN
-  return __builtin_bit_cast(u16, b);
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 
 // (m, s) pairs of an online log-sum-exp: s = sum exp(x - m)
 __device__ __forceinline__ void lse_combine(float& m, float& s, float m2, float s2) {
@@ -1019,20 +1000,12 @@ __global__ void __launch_bounds__(kBlock) state_digest_kernel(const DigestRow* _
   }
 }
 
-hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }
-
 void check_bf16(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
   TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16");
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
 }
-
-#define LAUNCH_CHECK()                                                                         \
-  do {                                                                                         \
-    hipError_t e_ = hipGetLastError();                                                         \
-    TORCH_CHECK(e_ == hipSuccess, "HIP launch failed: ", hipGetErrorString(e_));               \
-  } while (0)
 
 int vpl_for(int D) {
   const int nvec = D / 8;
@@ -1581,4 +1554,5 @@ PYBIND11_MODULE(_fused_ops, m) {
   m.def("swiglu_bwd", &swiglu_bwd);
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd", &ce_bwd);
+  register_rotary(m);
 }

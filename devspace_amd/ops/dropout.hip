@@ -1,0 +1,529 @@
+// Dropout for gfx950 whose mask is computed from a counter and never stored, alone, with the residual's
+// add, and with the residual's add and RMSNorm.
+//
+//   keep(row, col) <=> word[col % 4] of Philox(key = seed, counter = (col / 4, row, row >> 32, offset))
+//                      >= round(p 2^32)
+//   dropout               y = keep ? x / (1 - p) : 0
+//   dropout_add           s = x + dropout(delta)
+//   dropout_add_rms_norm  s as above, y = s r w, r = rsqrt(mean s^2 + eps)
+//   backward of the last  g = ds + r w dy - s r^3 / D sum(w dy s), dx = g, ddelta = dropout(g),
+//                         dw = sum over rows of dy s r
+//
+// Philox 4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3",
+// 2011): the backward pass computes the same words again instead of reading a mask. A block of four words
+// belongs to four neighbouring columns of a row, so that eight elements (one access of 16 bytes in 16-bit
+// types) are two blocks whatever the row's length. All of a row's math is in fp32; each output is rounded
+// once, and y is made of the sum before its rounding.
+#include "fused_common.h"
+
+#include <algorithm>
+#include <vector>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int64_t kMaxNormDim = 16384;
+
+struct Drop {
+  const int64_t* seed_at;  // null: seed
+  uint64_t seed;
+  unsigned offset;
+  unsigned last;  // the largest dropped word
+  bool none;      // p rounds to 0: nothing is dropped
+  float scale;    // 1 / (1 - p); 0 where p is 1
+};
+
+struct Key {
+  unsigned k0, k1, offset, last;
+  bool none;
+  float scale;
+  __device__ __forceinline__ explicit Key(const Drop& d) : offset(d.offset), last(d.last), none(d.none), scale(d.scale) {
+    const uint64_t s = d.seed_at ? (uint64_t)*d.seed_at : d.seed;
+    k0 = (unsigned)s;
+    k1 = (unsigned)(s >> 32);
+  }
+};
+
+__device__ __forceinline__ void philox(unsigned c0, unsigned c1, unsigned c2, unsigned c3, unsigned k0, unsigned k1,
+                                       unsigned w[4]) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+    c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+    c1 = (unsigned)b;
+    c3 = (unsigned)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  w[0] = c0, w[1] = c1, w[2] = c2, w[3] = c3;
+}
+
+// The eight elements at column 8 v of a row, kept and scaled or dropped. What is dropped becomes 0
+// whatever it was (a product with the mask would make NaN of an infinity).
+__device__ __forceinline__ void drop8(float f[8], int64_t row, unsigned v, const Key& k) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    unsigned w[4];
+    philox(2 * v + q, (unsigned)row, (unsigned)((uint64_t)row >> 32), k.offset, k.k0, k.k1, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[4 * q + i] = (w[i] > k.last || k.none) ? f[4 * q + i] * k.scale : 0.f;
+  }
+}
+
+// Up to eight elements of a row: one wide access, or the tail element by element.
+template <typename E>
+__device__ __forceinline__ void load8(const typename E::S* p, int n, float f[8]) {
+  if (n >= 8) {
+    const auto x = load_pack<typename E::S, 8>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = E::get(x.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < n ? E::get(p[i]) : 0.f;
+  }
+}
+template <typename E>
+__device__ __forceinline__ void store8(typename E::S* p, int n, const float f[8]) {
+  if (n >= 8) {
+    Pack<typename E::S, 8> x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.v[i] = E::put(f[i]);
+    store_pack<typename E::S, 8>(p, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = E::put(f[i]);
+  }
+}
+
+// ------------------------------------------------------------------------------ dropout, dropout + add
+
+// y = [x +] drop(d). Eight elements per work item; a launch covers rows row0.. with fewer than 2^31 items.
+template <typename E, bool ADD>
+__global__ void __launch_bounds__(kThreads) dropout_kernel(const typename E::S* __restrict__ d,
+                                                           const typename E::S* __restrict__ x,
+                                                           typename E::S* __restrict__ y, unsigned items, int64_t row0,
+                                                           int D, FastDiv by_row, Drop drop) {
+  const Key key(drop);
+  for (unsigned u = blockIdx.x * kThreads + threadIdx.x; u < items; u += gridDim.x * kThreads) {
+    unsigned v;
+    const unsigned r = by_row.divmod(u, v);
+    const int64_t row = row0 + r;
+    const int64_t at = row * D + 8 * (int64_t)v;
+    const int n = D - 8 * (int)v;
+    float f[8], g[8];
+    load8<E>(d + at, n, f);
+    if (ADD) load8<E>(x + at, n, g);
+    drop8(f, row, v, key);
+    if (ADD) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] += g[i];
+    }
+    store8<E>(y + at, n, f);
+  }
+}
+
+// ------------------------------------------------------------------------------ dropout + add + norm
+
+// Sum over the lanes that share a row: a wave, or the block's four waves through LDS.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = wave_sum(v);
+  if (LANES == 64) return v;
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();  // the last row's sums have been read
+  if ((threadIdx.x & 63) == 0) red[wave] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// LANES lanes per row (64 or 256), VPL groups of eight elements per lane: lane l owns groups l, l + LANES, ...
+// and keeps them in registers between the sum of squares and the scaled store, so that each tensor passes once.
+template <typename E, int LANES, int VPL>
+__global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename E::S* __restrict__ x,
+                                                                 const typename E::S* __restrict__ delta,
+                                                                 const typename E::S* __restrict__ w,
+                                                                 typename E::S* __restrict__ sum,
+                                                                 typename E::S* __restrict__ y, float* __restrict__ rstd,
+                                                                 int64_t R, int D, float eps, Drop drop) {
+  __shared__ float red[4];
+  const int lane = LANES == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const int64_t row = LANES == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (LANES == 64 && row >= R) return;
+  const Key key(drop);
+  const int nvec = (D + 7) >> 3;
+  const int64_t base = row * D;
+  float s[VPL][8], d[VPL][8];
+#pragma unroll
+  for (int k = 0; k < VPL; ++k) {
+    const int i = lane + LANES * k;
+    if (i < nvec) {
+      load8<E>(x + base + 8 * i, D - 8 * i, s[k]);
+      load8<E>(delta + base + 8 * i, D - 8 * i, d[k]);
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < VPL; ++k) {
+    const int i = lane + LANES * k;
+    if (i < nvec) {
+      drop8(d[k], row, i, key);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[k][j] += d[k][j];
+        ss += s[k][j] * s[k][j];  // columns behind the row are 0
+      }
+      store8<E>(sum + base + 8 * i, D - 8 * i, s[k]);
+    }
+  }
+  ss = row_sum<LANES>(ss, red);
+  const float r = rsqrtf(ss / (float)D + eps);
+  if (lane == 0) rstd[row] = r;
+#pragma unroll
+  for (int k = 0; k < VPL; ++k) {
+    const int i = lane + LANES * k;
+    if (i < nvec) {
+      float wv[8];
+      load8<E>(w + 8 * i, D - 8 * i, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[k][j] *= r * wv[j];
+      store8<E>(y + base + 8 * i, D - 8 * i, s[k]);
+    }
+  }
+}
+
+// A block owns rows_per_block rows (with 64 lanes per row its four waves take turns); each lane adds the
+// weight gradient of its columns in registers, and the block writes one fp32 row of partial sums, which
+// col_sum_kernel adds in a fixed order.
+template <typename E, int LANES, int VPL>
+__global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
+    const typename E::S* __restrict__ dy, const typename E::S* __restrict__ ds, const typename E::S* __restrict__ s,
+    const typename E::S* __restrict__ w, const float* __restrict__ rstd, typename E::S* __restrict__ dx,
+    typename E::S* __restrict__ dd, float* __restrict__ part, int64_t R, int D, int rows_per_block, Drop drop) {
+  __shared__ float red[4];
+  extern __shared__ float sdw[];  // [4][D], with 64 lanes per row
+  const int lane = LANES == 64 ? threadIdx.x & 63 : threadIdx.x;
+  constexpr int kStep = LANES == 64 ? 4 : 1;
+  const Key key(drop);
+  const int nvec = (D + 7) >> 3;
+  float acc[VPL][8];
+#pragma unroll
+  for (int k = 0; k < VPL; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[k][j] = 0.f;
+  const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = min(R, r0 + rows_per_block);
+  const float inv_d = 1.0f / (float)D;
+  // kept in registers where they fit beside the weight gradient: the weight over all rows, and the residual's
+  // gradient from the row's first loads on
+  constexpr bool kKeepW = VPL <= 2, kEarly = VPL <= 4;
+  float wv[VPL][8], rv[VPL][8];
+  if (kKeepW) {
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) load8<E>(w + 8 * (lane + LANES * k), D - 8 * (lane + LANES * k), wv[k]);
+  }
+  for (int64_t row = r0 + (LANES == 64 ? threadIdx.x >> 6 : 0); row < r1; row += kStep) {
+    const int64_t base = row * D;
+    float g[VPL][8], sv[VPL][8];
+    float dot = 0.f;
+    const float r = rstd[row];
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int i = lane + LANES * k;
+      if (i < nvec) {
+        if (dy) load8<E>(dy + base + 8 * i, D - 8 * i, g[k]);
+        load8<E>(s + base + 8 * i, D - 8 * i, sv[k]);
+        if (kEarly && ds) load8<E>(ds + base + 8 * i, D - 8 * i, rv[k]);
+        if (!kKeepW) load8<E>(w + 8 * i, D - 8 * i, wv[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (!dy) g[k][j] = 0.f;
+          acc[k][j] += g[k][j] * sv[k][j] * r;
+          g[k][j] *= wv[k][j];
+          dot += g[k][j] * sv[k][j];
+        }
+      }
+    }
+    dot = row_sum<LANES>(dot, red);
+    const float c = dot * r * r * r * inv_d;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int i = lane + LANES * k;
+      if (i < nvec) {
+        if (!kEarly && ds) load8<E>(ds + base + 8 * i, D - 8 * i, rv[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[k][j] = r * g[k][j] - sv[k][j] * c + (ds ? rv[k][j] : 0.f);
+        store8<E>(dx + base + 8 * i, D - 8 * i, g[k]);
+        drop8(g[k], row, i, key);
+        store8<E>(dd + base + 8 * i, D - 8 * i, g[k]);
+      }
+    }
+  }
+  float* out = part + (int64_t)blockIdx.x * D;
+  if (LANES == 64) {
+    float* mine = sdw + (threadIdx.x >> 6) * D;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int i = lane + LANES * k;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (8 * i + j < D) mine[8 * i + j] = acc[k][j];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < D; c += kThreads) out[c] = (sdw[c] + sdw[D + c]) + (sdw[2 * D + c] + sdw[3 * D + c]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      const int i = lane + LANES * k;
+      if (i < nvec) store8<FP32>(out + 8 * i, D - 8 * i, acc[k]);
+    }
+  }
+}
+
+// out[c] = sum over rows of part[row][c]: 32 columns per block, 32 groups of rows, added in a fixed order.
+template <typename E>
+__global__ void __launch_bounds__(1024) part_sum_kernel(const float* __restrict__ part, int rows, int D,
+                                                        typename E::S* __restrict__ out) {
+  __shared__ float red[32][33];
+  const int cl = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + cl;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < D) {
+    int r = g;
+    for (; r + 3 * 32 < rows; r += 4 * 32) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += part[(int64_t)(r + 32 * u) * D + c];
+    }
+    for (; r < rows; r += 32) s[0] += part[(int64_t)r * D + c];
+  }
+  red[g][cl] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (threadIdx.x < 32 && c < D) {
+    float t = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < 32; ++k) t += red[k][cl];
+    out[c] = E::put(t);
+  }
+}
+
+// ------------------------------------------------------------------------------ host side
+
+Drop make_drop(double p, int64_t seed, const c10::optional<at::Tensor>& seed_at, int64_t offset) {
+  Drop d{};
+  d.seed = (uint64_t)seed;
+  if (seed_at) d.seed_at = seed_at->data_ptr<int64_t>();
+  d.offset = (unsigned)offset;
+  const double words = std::nearbyint(p * 4294967296.0);  // words below this one are dropped
+  d.none = words < 1.0;
+  d.last = d.none ? 0u : (unsigned)(words - 1.0);
+  d.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
+  return d;
+}
+
+void check_drop(const char* op, const at::Tensor& x, double p, const c10::optional<at::Tensor>& seed_at, int64_t offset) {
+  TORCH_CHECK(x.is_cuda(), op, ": GPU tensors wanted");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf || x.scalar_type() == at::kFloat, op,
+              ": bfloat16, float16 or float32 wanted");
+  TORCH_CHECK(p >= 0.0 && p <= 1.0, op, ": p must be within 0 and 1");
+  TORCH_CHECK(offset >= 0 && offset < (1ll << 32), op, ": offset must be within 0 and 2^32 - 1");
+  TORCH_CHECK(!seed_at || (seed_at->scalar_type() == at::kLong && seed_at->numel() == 1 && seed_at->device() == x.device()),
+              op, ": a seed tensor must hold one int64 on the device of the data");
+  TORCH_CHECK(x.dim() == 0 || x.size(-1) < (1ll << 31) - 8, op, ": rows of fewer than 2^31 elements wanted");
+}
+
+void same(const char* op, const char* name, const at::Tensor& a, const at::Tensor& b) {
+  TORCH_CHECK(a.sizes() == b.sizes() && a.scalar_type() == b.scalar_type() && a.device() == b.device(), op, ": ", name,
+              " must agree in shape, type and device");
+}
+
+template <typename F>
+void by_type(at::ScalarType t, F&& f) {
+  switch (t) {
+    case at::kBFloat16: f(BF16{}); break;
+    case at::kHalf: f(FP16{}); break;
+    default: f(FP32{}); break;
+  }
+}
+
+// drop(d), or x + drop(d); contiguous inputs
+at::Tensor dropout_apply(const at::Tensor& d, const at::Tensor& x, const Drop& drop) {
+  c10::DeviceGuard guard(d.device());
+  auto y = at::empty_like(d);
+  if (d.numel() == 0) return y;
+  const int64_t D = d.dim() ? d.size(-1) : 1, R = d.numel() / D, nvec = (D + 7) / 8;
+  const int64_t most = std::max<int64_t>(1, ((1ll << 30)) / nvec);  // rows of one launch: items stay under 2^31
+  for (int64_t r0 = 0; r0 < R; r0 += most) {
+    const int64_t items = std::min(most, R - r0) * nvec;
+    const unsigned blocks = (unsigned)((items + kThreads - 1) / kThreads);
+    by_type(d.scalar_type(), [&](auto e) {
+      typedef decltype(e) E;
+      typedef typename E::S S;
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, stream(), (const S*)d.data_ptr(),
+                           x.defined() ? (const S*)x.data_ptr() : nullptr, (S*)y.data_ptr(), (unsigned)items, r0, (int)D,
+                           FastDiv((unsigned)nvec), drop);
+      };
+      x.defined() ? go(dropout_kernel<E, true>) : go(dropout_kernel<E, false>);
+    });
+    LAUNCH_CHECK();
+  }
+  return y;
+}
+
+// Lanes per row and groups per lane of the norm kernels: a wave per row up to 2048 columns (no barrier, four
+// rows in flight per block), the whole block beyond.
+template <typename F>
+void by_width(int64_t D, F&& f) {
+  using std::integral_constant;
+  const int64_t n = (D + 7) / 8;
+  if (n <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (n <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (n <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  else if (n <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (n <= 1024) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  else f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+}
+
+struct NormForward {
+  at::Tensor sum, y, rstd;
+};
+
+NormForward drop_norm_fwd(const at::Tensor& x, const at::Tensor& delta, const at::Tensor& w, double eps, const Drop& drop) {
+  c10::DeviceGuard guard(x.device());
+  const int64_t D = x.size(-1), R = D ? x.numel() / D : 0;
+  NormForward o{at::empty_like(x), at::empty_like(x), at::empty({R}, x.options().dtype(at::kFloat))};
+  if (R == 0) return o;
+  by_type(x.scalar_type(), [&](auto e) {
+    typedef decltype(e) E;
+    typedef typename E::S S;
+    by_width(D, [&](auto lanes, auto vpl) {
+      const int64_t blocks = lanes == 64 ? (R + 3) / 4 : R;
+      TORCH_CHECK(blocks < (1ll << 31), "dropout_add_rms_norm: too many rows");
+      hipLaunchKernelGGL((drop_norm_fwd_kernel<E, lanes, vpl>), dim3((unsigned)blocks), dim3(kThreads), 0, stream(),
+                         (const S*)x.data_ptr(), (const S*)delta.data_ptr(), (const S*)w.data_ptr(), (S*)o.sum.data_ptr(),
+                         (S*)o.y.data_ptr(), o.rstd.data_ptr<float>(), R, (int)D, (float)eps, drop);
+    });
+  });
+  LAUNCH_CHECK();
+  return o;
+}
+
+// dy or ds may be undefined (zero)
+std::vector<at::Tensor> drop_norm_bwd(const at::Tensor& dy, const at::Tensor& ds, const at::Tensor& s, const at::Tensor& w,
+                                      const at::Tensor& rstd, const Drop& drop) {
+  c10::DeviceGuard guard(s.device());
+  const int64_t D = s.size(-1), R = D ? s.numel() / D : 0;
+  auto dx = at::empty_like(s), dd = at::empty_like(s), dw = at::empty_like(w);
+  if (R == 0) return {dx, dd, dw.zero_()};
+  by_type(s.scalar_type(), [&](auto e) {
+    typedef decltype(e) E;
+    typedef typename E::S S;
+    by_width(D, [&](auto lanes, auto vpl) {
+      // two rows per wave, or per block; at most 1024 rows of partial sums
+      const int64_t at_once = lanes == 64 ? 4 : 1;
+      const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(1024, (R + 2 * at_once - 1) / (2 * at_once)));
+      const int64_t per = (R + blocks - 1) / blocks;
+      TORCH_CHECK(per < (1ll << 31), "dropout_add_rms_norm: too many rows");
+      auto part = at::empty({blocks, D}, s.options().dtype(at::kFloat));
+      hipLaunchKernelGGL((drop_norm_bwd_kernel<E, lanes, vpl>), dim3((unsigned)blocks), dim3(kThreads),
+                         lanes == 64 ? 4 * D * sizeof(float) : 0, stream(), dy.defined() ? (const S*)dy.data_ptr() : nullptr,
+                         ds.defined() ? (const S*)ds.data_ptr() : nullptr, (const S*)s.data_ptr(), (const S*)w.data_ptr(),
+                         rstd.data_ptr<float>(), (S*)dx.data_ptr(), (S*)dd.data_ptr(), part.data_ptr<float>(), R, (int)D,
+                         (int)per, drop);
+      LAUNCH_CHECK();
+      hipLaunchKernelGGL((part_sum_kernel<E>), dim3((unsigned)((D + 31) / 32)), dim3(1024), 0, stream(),
+                         part.data_ptr<float>(), (int)blocks, (int)D, (S*)dw.data_ptr());
+      LAUNCH_CHECK();
+    });
+  });
+  return {dx, dd, dw};
+}
+
+// ------------------------------------------------------------------------------ autograd
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef c10::optional<at::Tensor> OptTensor;
+
+void no_second_order(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": second derivatives are not implemented");
+}
+
+void save_drop(AutogradContext* ctx, double p, int64_t seed, int64_t offset) {
+  ctx->saved_data["p"] = p;
+  ctx->saved_data["seed"] = seed;
+  ctx->saved_data["offset"] = offset;
+}
+Drop saved_drop(AutogradContext* ctx, const at::Tensor& seed_at) {
+  OptTensor t;
+  if (seed_at.defined()) t = seed_at;
+  return make_drop(ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), t, ctx->saved_data["offset"].toInt());
+}
+
+struct DropoutFn : public torch::autograd::Function<DropoutFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& d, const OptTensor& x, double p, int64_t seed,
+                            const OptTensor& seed_at, int64_t offset) {
+    ctx->save_for_backward({seed_at ? *seed_at : at::Tensor()});
+    save_drop(ctx, p, seed, offset);
+    ctx->saved_data["add"] = x.has_value();
+    return dropout_apply(d.contiguous(), x ? x->contiguous() : at::Tensor(), make_drop(p, seed, seed_at, offset));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_second_order("dropout");
+    at::Tensor none, seed_at = ctx->get_saved_variables()[0], dd;
+    if (ctx->needs_input_grad(0)) dd = dropout_apply(grads[0].contiguous(), none, saved_drop(ctx, seed_at));
+    return {dd, ctx->saved_data["add"].toBool() ? grads[0] : none, none, none, none, none};
+  }
+};
+
+struct DropNormFn : public torch::autograd::Function<DropNormFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& delta, const at::Tensor& w,
+                               double eps, double p, int64_t seed, const OptTensor& seed_at, int64_t offset) {
+    auto wc = w.contiguous();
+    auto o = drop_norm_fwd(x.contiguous(), delta.contiguous(), wc, eps, make_drop(p, seed, seed_at, offset));
+    ctx->save_for_backward({o.sum, wc, o.rstd, seed_at ? *seed_at : at::Tensor()});
+    save_drop(ctx, p, seed, offset);
+    ctx->set_materialize_grads(false);
+    return {o.sum, o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_second_order("dropout_add_rms_norm");
+    auto s = ctx->get_saved_variables();
+    auto dense = [](const at::Tensor& g) { return g.defined() ? g.contiguous() : g; };
+    at::Tensor none;
+    if (!grads[0].defined() && !grads[1].defined()) return {none, none, none, none, none, none, none, none};
+    auto r = drop_norm_bwd(dense(grads[1]), dense(grads[0]), s[0], s[1], s[2], saved_drop(ctx, s[3]));
+    return {r[0], r[1], r[2], none, none, none, none, none};
+  }
+};
+
+at::Tensor dropout(const at::Tensor& d, const OptTensor& x, double p, int64_t seed, const OptTensor& seed_at,
+                   int64_t offset) {
+  const char* op = x ? "dropout_add" : "dropout";
+  check_drop(op, d, p, seed_at, offset);
+  if (x) same(op, "x and delta", *x, d);
+  if (at::GradMode::is_enabled() && (d.requires_grad() || (x && x->requires_grad())))
+    return DropoutFn::apply(d, x, p, seed, seed_at, offset);
+  return dropout_apply(d.contiguous(), x ? x->contiguous() : at::Tensor(), make_drop(p, seed, seed_at, offset));
+}
+
+std::vector<at::Tensor> dropout_add_rms_norm(const at::Tensor& x, const at::Tensor& delta, const at::Tensor& w, double eps,
+                                             double p, int64_t seed, const OptTensor& seed_at, int64_t offset) {
+  const char* op = "dropout_add_rms_norm";
+  check_drop(op, x, p, seed_at, offset);
+  same(op, "x and delta", x, delta);
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) <= kMaxNormDim, op, ": rows of at most ", kMaxNormDim, " elements wanted");
+  TORCH_CHECK(w.dim() == 1 && w.numel() == x.size(-1) && w.scalar_type() == x.scalar_type() && w.device() == x.device(), op,
+              ": weight must be [D], of the data's type and device");
+  if (at::GradMode::is_enabled() && (x.requires_grad() || delta.requires_grad() || w.requires_grad()))
+    return DropNormFn::apply(x, delta, w, eps, p, seed, seed_at, offset);
+  auto o = drop_norm_fwd(x.contiguous(), delta.contiguous(), w.contiguous(), eps, make_drop(p, seed, seed_at, offset));
+  return {o.sum, o.y};
+}
+
+}  // namespace
+
+void register_dropout(pybind11::module_& m) {
+  m.def("dropout", &dropout, "dropout(delta), or x + dropout(delta), from a seed, an optional seed tensor and an offset");
+  m.def("dropout_add_rms_norm", &dropout_add_rms_norm, "(s, y): s = x + dropout(delta), y = rmsnorm(s) * w");
+}

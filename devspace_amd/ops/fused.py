@@ -6,6 +6,7 @@
     y = fused.swiglu(h)                   # silu(h[..., :H]) * h[..., H:]
     loss = fused.cross_entropy(logits, t) # mean CE on bf16 logits [N, V]
     qkv = fused.rotary_qkv(qkv, positions, freqs)     # q and k turned by their positions
+    x, h = fused.dropout_add_rms_norm(x, delta, norm.weight, p, seed)  # no mask is stored
 
 On a GPU the HIP kernels are mandatory: if the in-tree extension is missing or broken the
 first call raises (no silent eager fallback). On CPU tensors (tests, CPU smoke runs) the plain
@@ -313,6 +314,106 @@ class Rotary(nn.Module):
         if k is None:
             return rotary_qkv(q, positions, self.freqs, self.interleaved, self.magnitude)
         return rotary_qk(q, k, positions, self.freqs, self.interleaved, self.magnitude)
+
+
+# ------------------------------------------------------------------------------ dropout
+
+
+def _check_dropout(op, p, seed, offset):
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{op}: p must be within 0 and 1")
+    if not 0 <= offset < 1 << 32:
+        raise ValueError(f"{op}: offset must be within 0 and 2^32 - 1")
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError(f"{op}: a seed tensor must hold one int64")
+        return 0, seed
+    if not -(1 << 63) <= seed < 1 << 64:
+        raise ValueError(f"{op}: seed must fit 64 bits")
+    return (int(seed) + (1 << 63)) % (1 << 64) - (1 << 63), None  # the same 64 bits with a sign
+
+
+def _dropout_factor(shape, p, seed, offset, device):
+    """1 / (1 - p) where an element of `shape` stays and 0 where it is dropped (float64): the words of
+    Philox 4x32-10 in PyTorch ops, the gfx950 kernels' own."""
+    low = (1 << 32) - 1
+    d = shape[-1] if len(shape) else 1
+    rows = math.prod(shape[:-1])
+    c0 = torch.arange((d + 3) // 4, device=device).expand(rows, -1)
+    row = torch.arange(rows, device=device)[:, None].expand_as(c0)
+    c1, c2, c3 = row & low, row >> 32, torch.full_like(c0, offset)
+    k0, k1 = seed & low, (seed >> 32) & low
+    for _ in range(10):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # modulo 2^64: both halves are right
+        c0, c1, c2, c3 = ((b >> 32) & low) ^ c1 ^ k0, b & low, ((a >> 32) & low) ^ c3 ^ k1, a & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    words = torch.stack((c0, c1, c2, c3), -1).flatten(1)[:, :d].reshape(shape)
+    return (words >= round(p * 2.0 ** 32)).double() * (1.0 / (1.0 - p) if p < 1.0 else 0.0)
+
+
+def _dropped(x, p, seed, seed_at, offset):
+    """x dropped and scaled, unrounded (float32, or float64 for float64)."""
+    factor = _dropout_factor(x.shape, p, int(seed_at) if seed_at is not None else seed, offset, x.device)
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    return torch.where(factor != 0, x.to(wide) * factor.to(wide), torch.zeros((), dtype=wide, device=x.device))
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
+    """x with each element dropped with probability p, the others divided by 1 - p. The mask is a
+    function of (seed, offset, row, column) of x seen as [rows, last dimension]; it is computed again
+    in the backward pass and never stored. Dropped elements are 0, whatever they were.
+
+    seed: a whole number of 64 bits, or a tensor of one int64 on the data's device (a captured graph
+    reads it anew at each replay; it must not change between a forward pass and its backward pass).
+    offset: 0 to 2^32 - 1, to tell the dropouts of one step apart. The masks are the same on every device."""
+    seed, at = _check_dropout("dropout", p, seed, offset)
+    if x.is_cuda and x.dtype in _HIP_FLOATS:
+        return ext().dropout(x, None, float(p), seed, at, offset)
+    return _dropped(x, p, seed, at, offset).to(x.dtype)
+
+
+def dropout_add(x: torch.Tensor, delta: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
+    """x + dropout(delta, p, seed, offset) in one kernel, rounded once."""
+    seed, at = _check_dropout("dropout_add", p, seed, offset)
+    if x.shape != delta.shape or x.dtype != delta.dtype or x.device != delta.device:
+        raise ValueError("dropout_add: x and delta must agree in shape, type and device")
+    if x.is_cuda and x.dtype in _HIP_FLOATS:
+        return ext().dropout(delta, x, float(p), seed, at, offset)
+    return (x + _dropped(delta, p, seed, at, offset)).to(x.dtype)
+
+
+def dropout_add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, p: float, seed,
+                         eps: float | None = None, offset: int = 0):
+    """add_rms_norm() of a residual stream with dropout: returns (s, y) with
+    s = x + dropout(delta, p, seed, offset) and y = rms_norm(s) * weight, one kernel each way (and a
+    small one for the weight's gradient). y is made of the sum before it is rounded to s."""
+    seed, at = _check_dropout("dropout_add_rms_norm", p, seed, offset)
+    if x.shape != delta.shape or x.dtype != delta.dtype or x.device != delta.device:
+        raise ValueError("dropout_add_rms_norm: x and delta must agree in shape, type and device")
+    if x.dim() < 1 or weight.shape != x.shape[-1:] or weight.dtype != x.dtype:
+        raise ValueError("dropout_add_rms_norm: weight must be [D] and of the data's type")
+    if eps is None:
+        eps = torch.finfo(x.dtype).eps
+    if x.is_cuda and x.dtype in _HIP_FLOATS:
+        return tuple(ext().dropout_add_rms_norm(x, delta, weight, float(eps), float(p), seed, at, offset))
+    s = x + _dropped(delta, p, seed, at, offset)
+    return s.to(x.dtype), (s * torch.rsqrt(s.square().mean(-1, keepdim=True) + eps) * weight).to(x.dtype)
+
+
+class Dropout(nn.Module):
+    """nn.Dropout(p) on the fused kernels. Each call takes its seed from PyTorch's CPU generator (so
+    torch.manual_seed and checkpointed recomputation repeat it); `residual` is added in the same kernel."""
+
+    def __init__(self, p: float = 0.5):
+        super().__init__()
+        _check_dropout("Dropout", p, 0, 0)
+        self.p = p
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0.0:
+            return x if residual is None else residual + x
+        seed = int(torch.randint(-(1 << 63), (1 << 63) - 1, ()))
+        return dropout(x, self.p, seed) if residual is None else dropout_add(residual, x, self.p, seed)
 
 
 # ------------------------------------------------------------------------------ AdamW

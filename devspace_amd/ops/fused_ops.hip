@@ -26,6 +26,7 @@
 #include <vector>
 
 void register_rotary(pybind11::module_& m);
+void register_dropout(pybind11::module_& m);
 
 namespace {
 
@@ -1555,4 +1556,5 @@ PYBIND11_MODULE(_fused_ops, m) {
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd", &ce_bwd);
   register_rotary(m);
+  register_dropout(m);
 }

@@ -12,7 +12,7 @@ import subprocess
 import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-FUSED_SOURCES = ("fused_ops.hip", "rotary.hip", "dropout.hip")
+FUSED_SOURCES = ("fused_ops.hip", "rotary.hip", "dropout.hip", "cross_attention.hip")
 FUSED_HEADERS = ("fused_common.h",)
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 # No packed fp32 instructions (v_pk_add/mul/fma_f32), which the compiler would otherwise make from

@@ -1,0 +1,894 @@
+// Cross attention for gfx950: queries of one sequence over the encoder's states of another length.
+//
+//   q [B, Tq, H, D], kv [B, Tk, 2, N, D] (packed keys and values, N divides H, G = H / N), len_b <= Tk states
+//   S = scale q k^T over the first len_b states, P = softmax(S), O = P V; len_b = 0: O = 0, gradients 0
+//   D_r = rowsum(dO * O), dV = P^T dO, dS = P * (dO V^T - D_r), dQ = scale dS K, dK = scale dS^T Q
+//
+// There is no causal mask, so the G query heads that share a key head are stacked: row m = t G + g, M = G Tq
+// rows over one set of keys, each key and value read once for all of them. All products run on
+// v_mfma_f32_32x32x16 (bf16 or fp16 in, fp32 out); softmax statistics and sums are in fp32. P and dS are
+// rounded to the 16-bit type as operands of the next product (half a step each, averaged over the keys),
+// as are the outputs; nothing else is.
+//
+//   cross_fwd_kernel   128 rows (4 waves x 32), key tiles of 64 double-buffered in LDS
+//   cross_few_kernel   up to 32 rows (single tokens): every wave goes through key tiles of its own, keys
+//                      straight into registers, values through a small LDS tile of the wave; joined in LDS
+//   cross_dq_kernel    128 rows over all key tiles; also D_r
+//   cross_dkv_kernel   128 keys over all row tiles; sums over a group's heads in registers, no atomics
+// Each can split its long axis over several workgroups where there are too few of them to fill the chip;
+// join kernels then add the parts in a fixed order.
+//
+// S is computed transposed (keys on the matrix rows, query rows on the lanes), so that a row's maximum and sum
+// are lane-local plus one exchange of the wave's halves, and the accumulators are the next product's operand
+// as they stand; V^T, K^T, Q^T and dO^T come from ds_read_b64_tr_b16 reads of row-major LDS tiles.
+#include "fused_common.h"
+
+#include <algorithm>
+#include <vector>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRows = 128;  // query rows (forward, dQ) or keys (dK, dV) of a workgroup: 32 per wave
+constexpr int kKeys = 64;   // keys of an LDS tile
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+
+template <typename E>
+__device__ __forceinline__ f32x16 mfma(const u16x8& a, const u16x8& b, const f32x16& c) {
+  if constexpr (E::kType == at::kBFloat16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// A tile's rows of D <= DP columns take RB bytes. 16-byte chunks are swizzled by the row: the row reads
+// (ds_read_b128, 16 rows of one chunk) and the transposed reads (4 neighbouring rows of 4 neighbouring chunks)
+// both fall on different banks.
+template <int DP>
+struct Tile {
+  static constexpr int RB = DP <= 64 ? 128 : 256;
+  static constexpr int CH = DP / 8;   // chunks of a row
+  static constexpr int KS = DP / 16;  // steps of a product over the columns
+  static constexpr int NB = DP / 32;  // blocks of 32 columns
+  __device__ static __forceinline__ int off(int row, int chunk) {
+    if constexpr (RB == 128) return row * 128 + ((chunk ^ ((row >> 1) & 7) ^ ((row & 2) << 1)) << 4);
+    else return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+  }
+  __device__ static __forceinline__ u16x8 row8(const unsigned char* tile, int row, int chunk) {
+    return *reinterpret_cast<const u16x8*>(tile + off(row, chunk));
+  }
+  // Operand of the transposed tile: lane (r = lane & 31, hh = lane >> 5) gets column col0 + r of rows
+  // r0 + 4 hh + {0..3} and r0 + 8 + 4 hh + {0..3}: the order of an accumulator's rows.
+  __device__ static __forceinline__ u16x8 tr8(const unsigned char* tile, int r0, int col0, int lane) {
+    const int g = lane >> 4, i = lane & 15, hh = lane >> 5;
+    const int row = r0 + 4 * hh + (i >> 2);
+    const int col = col0 + 16 * (g & 1) + 4 * (i & 3);
+    lds_u8* base = (lds_u8*)tile;
+    s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + off(row, col >> 3) + ((col & 7) << 1)));
+    s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + off(row + 8, col >> 3) + ((col & 7) << 1)));
+    return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// 2^x on the transcendental unit; 2^-inf = 0, which masked scores rely on
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename E>
+__device__ __forceinline__ u16x8 to_operand(const f32x16& acc, int s) {
+  u16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = E::put(acc[8 * s + j]);
+  return o;
+}
+
+// row of a 32x32 accumulator in register i of lane half hh
+__device__ __forceinline__ int acc_row(int i, int hh) { return (i & 3) + 8 * (i >> 2) + 4 * hh; }
+
+__device__ __forceinline__ u16x8 zero8() {
+  u16x8 z;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = 0;
+  return z;
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+struct CrossParams {
+  const u16 *q, *kv, *o, *dout;
+  u16 *out, *dkv;       // O or dQ [B, Tq, H, D]; [B, Tk, 2, N, D]
+  float *part;          // split forward: O's parts [split][B N][M][D]; split dQ, dK, dV: parts in the output's layout
+  float *part_ml;       // split forward: (m, l) of each part [split][B N][M]
+  float *lse, *delta;   // [B N][M]; lse in the log2 domain of the scaled scores
+  const void* lengths;  // null: Tk
+  int64_t qb, qt, qh;   // strides in elements
+  int64_t kb, kt, ks, kh;
+  int64_t out_numel, dkv_numel;  // a part's size in the gradients' layout
+  int B, N, G, M, Tq, Tk, D;
+  int splits, per_split;  // keys (forward, dQ) or rows (dK, dV) of a split: whole tiles
+  int blocks;             // workgroups along the rows or keys
+  FastDiv by_G;
+  float scale, scale_log2;
+  bool len64;
+
+  __device__ __forceinline__ int length(int b) const {
+    if (!lengths) return Tk;
+    const int64_t n = len64 ? static_cast<const int64_t*>(lengths)[b] : (int64_t)static_cast<const int*>(lengths)[b];
+    return (int)(n < 0 ? 0 : n > Tk ? Tk : n);
+  }
+  // offset of row m of key head n in [B, Tq, H, D] with these strides
+  __device__ __forceinline__ int64_t row_at(int m, int b, int n, int64_t sb, int64_t st, int64_t sh) const {
+    unsigned g;
+    const unsigned t = by_G.divmod((unsigned)m, g);
+    return b * sb + (int64_t)t * st + ((int64_t)n * G + g) * sh;
+  }
+  __device__ __forceinline__ int64_t dense_at(int m, int b, int n) const {
+    const int64_t H = (int64_t)N * G;
+    return row_at(m, b, n, Tq * H * D, H * D, D);
+  }
+};
+
+// Which work a workgroup has. Workgroups go to the 8 XCDs in turn; the ones of one key head (neighbours here)
+// are given to one XCD, whose L2 then serves its keys and values.
+struct Place {
+  int block, split, n, b, bn;
+  __device__ __forceinline__ explicit Place(const CrossParams& p) {
+    const unsigned total = gridDim.x, id = blockIdx.x;
+    const unsigned xcd = id & 7, slot = id >> 3, each = total >> 3, rest = total & 7;
+    unsigned w = xcd * each + min(xcd, rest) + slot;
+    block = w % p.blocks;
+    w /= p.blocks;
+    split = w % p.splits;
+    bn = w / p.splits;
+    n = bn % p.N;
+    b = bn / p.N;
+  }
+};
+
+// 256 threads carry one tile of ROWS rows of two tensors through registers into LDS; rows and columns
+// outside are 0 and never read.
+template <int DP, int ROWS>
+struct Stage {
+  typedef Tile<DP> L;
+  static constexpr int kEach = ROWS * L::CH;
+  static constexpr int kPer = 2 * kEach / kThreads;
+  static_assert(2 * kEach % kThreads == 0, "whole chunks per thread");
+  u16x8 r[kPer];
+  template <typename F>
+  __device__ __forceinline__ void load(F&& at, int D) {  // at(which, row): the row's first element, or null
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int c = threadIdx.x + kThreads * u;
+      const int which = c >= kEach, cc = c - which * kEach;
+      const int row = cc / L::CH, ch = cc % L::CH;
+      const u16* src = ch * 8 < D ? at(which, row) : nullptr;
+      r[u] = src ? *reinterpret_cast<const u16x8*>(src + ch * 8) : zero8();
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* ta, unsigned char* tb) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int c = threadIdx.x + kThreads * u;
+      const int which = c >= kEach, cc = c - which * kEach;
+      *reinterpret_cast<u16x8*>((which ? tb : ta) + L::off(cc / L::CH, cc % L::CH)) = r[u];
+    }
+  }
+};
+
+// this lane's half of a row as KS operands (columns 16 s + 8 hh ..); null: zeros
+template <int DP>
+__device__ __forceinline__ void load_row(u16x8* f, const u16* row, int hh, int D) {
+#pragma unroll
+  for (int s = 0; s < Tile<DP>::KS; ++s) {
+    const int col = 16 * s + 8 * hh;
+    f[s] = row && col < D ? *reinterpret_cast<const u16x8*>(row + col) : zero8();
+  }
+}
+
+// One tile of scores in the log2 domain: the online softmax of this lane's row. On return s holds P.
+template <int KB>
+__device__ __forceinline__ float soften(f32x16* s, float& m, float& l, float scale_log2) {
+  float mt = -INFINITY;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
+  mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+  const float mn = fmaxf(m, mt * scale_log2);
+  const float base = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: all of P is 0
+  const float alpha = exp2_fast(m - base);
+  float ls = 0.f;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = exp2_fast(__builtin_fmaf(s[kb][i], scale_log2, -base));
+      s[kb][i] = e;
+      ls += e;
+    }
+  l = l * alpha + ls;
+  m = mn;
+  return alpha;
+}
+
+// Four columns of a row of O^T or dQ^T accumulators at a time: column nb 32 + 8 g4 + 4 hh
+template <int DP, typename F>
+__device__ __forceinline__ void each_quad(int hh, int D, F&& f) {
+#pragma unroll
+  for (int nb = 0; nb < Tile<DP>::NB; ++nb)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const int col = nb * 32 + 8 * g4 + 4 * hh;
+      if (col < D) f(col, nb, 4 * g4);
+    }
+}
+template <typename E>
+__device__ __forceinline__ void put4(u16* at, const f32x16& a, int i, float by) {
+  u16v<4> o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = E::put(a[i + j] * by);
+  *reinterpret_cast<u16v<4>*>(at) = o;
+}
+__device__ __forceinline__ void put4f(float* at, const f32x16& a, int i, float by) {
+  *reinterpret_cast<float4*>(at) = make_float4(a[i] * by, a[i + 1] * by, a[i + 2] * by, a[i + 3] * by);
+}
+
+// ------------------------------------------------------------------------------ forward
+
+template <typename E, int DP>
+__global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
+  typedef Tile<DP> L;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2][2][kKeys * L::RB];  // [buffer][K | V]
+  const Place w(p);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 31, hh = lane >> 5;
+  const int m0 = w.block * kRows + wave * 32, row = m0 + r;
+  const bool some = m0 < p.M;  // the wave has rows at all
+  const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
+  const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh;
+  u16x8 qf[L::KS];
+  load_row<DP>(qf, row < p.M ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
+  f32x16 o[L::NB];
+#pragma unroll
+  for (int nb = 0; nb < L::NB; ++nb) o[nb] = zero16();
+  float m = -INFINITY, l = 0.f;
+  Stage<DP, kKeys> stage;
+  auto load = [&](int k0) {
+    stage.load([&](int which, int i) { return k0 + i < k_end ? kbase + (int64_t)(k0 + i) * p.kt + which * p.ks : nullptr; }, p.D);
+  };
+  if (k_begin < k_end) {
+    load(k_begin);
+    stage.store(smem[0][0], smem[0][1]);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += kKeys, buf ^= 1) {
+    const bool more = k0 + kKeys < k_end;
+    if (more) load(k0 + kKeys);
+    const unsigned char *Ks = smem[buf][0], *Vs = smem[buf][1];
+    if (some) {
+      f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+      for (int st = 0; st < L::KS; ++st)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) s[kb] = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s[kb]);
+      if (k0 + kKeys > k_end) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (k0 + kb * 32 + acc_row(i, hh) >= k_end) s[kb][i] = -INFINITY;
+      }
+      const float alpha = soften<2>(s, m, l, p.scale_log2);
+#pragma unroll
+      for (int nb = 0; nb < L::NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const u16x8 pb = to_operand<E>(s[ks >> 1], ks & 1);
+#pragma unroll
+        for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(L::tr8(Vs, 16 * ks, nb * 32, lane), pb, o[nb]);
+      }
+    }
+    if (more) stage.store(smem[buf ^ 1][0], smem[buf ^ 1][1]);
+    __syncthreads();
+  }
+  if (row >= p.M) return;
+  l += __shfl_xor(l, 32, 64);
+  const int64_t stat = (int64_t)w.bn * p.M + row;
+  if (p.splits == 1) {
+    const float inv = k_begin < k_end ? 1.f / l : 0.f;  // no state at all: 0
+    u16* at = p.out + p.dense_at(row, w.b, w.n);
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4<E>(at + col, o[nb], i, inv); });
+    if (p.lse && hh == 0) p.lse[stat] = m + __log2f(l);
+  } else if (k_begin < k_end) {
+    const int64_t at = ((int64_t)w.split * p.B * p.N + w.bn) * p.M + row;
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4f(p.part + at * p.D + col, o[nb], i, 1.f); });
+    if (hh == 0) {
+      p.part_ml[2 * at] = m;
+      p.part_ml[2 * at + 1] = l;
+    }
+  }
+}
+
+// Up to 32 rows: wave w takes the 32-key tiles w, w + 4, ... of the split.
+template <typename E, int DP>
+__global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
+  typedef Tile<DP> L;
+  constexpr int kTile = 32;
+  constexpr int kPer = kTile * L::CH / 64;  // chunks of V per lane
+  __shared__ __attribute__((aligned(16))) union {
+    unsigned char v[4][kTile * L::RB];
+    float o[4][32][DP];
+  } sm;
+  __shared__ float sml[4][2][32];
+  const Place w(p);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 31, hh = lane >> 5;
+  const int m0 = w.block * 32, row = m0 + r;
+  const int rows = min(32, p.M - m0);
+  const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
+  const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh;
+  u16x8 qf[L::KS], kf[L::KS], vr[kPer];
+  load_row<DP>(qf, row < p.M ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
+  f32x16 o[L::NB];
+#pragma unroll
+  for (int nb = 0; nb < L::NB; ++nb) o[nb] = zero16();
+  float m = -INFINITY, l = 0.f;
+  unsigned char* Vs = sm.v[wave];
+  auto load_k = [&](int k0) {
+    load_row<DP>(kf, k0 + r < k_end ? kbase + (int64_t)(k0 + r) * p.kt : nullptr, hh, p.D);
+  };
+  auto load_v = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int c = lane + 64 * u, key = k0 + c / L::CH, ch = c % L::CH;
+      vr[u] = key < k_end && ch * 8 < p.D ? *reinterpret_cast<const u16x8*>(kbase + (int64_t)key * p.kt + p.ks + ch * 8) : zero8();
+    }
+  };
+  int k0 = k_begin + wave * kTile;
+  if (k0 < k_end) {
+    load_k(k0);
+    load_v(k0);
+  }
+  for (; k0 < k_end; k0 += 4 * kTile) {
+    const int next = k0 + 4 * kTile;
+    f32x16 s = zero16();
+#pragma unroll
+    for (int st = 0; st < L::KS; ++st) s = mfma<E>(kf[st], qf[st], s);
+    if (next < k_end) load_k(next);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int c = lane + 64 * u;
+      *reinterpret_cast<u16x8*>(Vs + L::off(c / L::CH, c % L::CH)) = vr[u];
+    }
+    if (next < k_end) load_v(next);
+    if (k0 + kTile > k_end) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + acc_row(i, hh) >= k_end) s[i] = -INFINITY;
+    }
+    const float alpha = soften<1>(&s, m, l, p.scale_log2);
+#pragma unroll
+    for (int nb = 0; nb < L::NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
+    // the tile belongs to this wave alone, and a wave's LDS operations stay in order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const u16x8 pb = to_operand<E>(s, ks);
+#pragma unroll
+      for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(L::tr8(Vs, 16 * ks, nb * 32, lane), pb, o[nb]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  // join the four waves: their maxima and sums, then their rows on the common maximum
+  l += __shfl_xor(l, 32, 64);
+  if (hh == 0) {
+    sml[wave][0][r] = m;
+    sml[wave][1][r] = l;
+  }
+  __syncthreads();  // the tiles are done with: their memory takes the rows
+  float mj = fmaxf(fmaxf(sml[0][0][r], sml[1][0][r]), fmaxf(sml[2][0][r], sml[3][0][r]));
+  const float base = mj == -INFINITY ? 0.f : mj;
+  float lj = 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) lj += sml[v][1][r] * exp2_fast(sml[v][0][r] - base);
+  const float mine = exp2_fast(m - base);
+  if (r < rows) each_quad<DP>(hh, DP, [&](int col, int nb, int i) { put4f(&sm.o[wave][r][col], o[nb], i, mine); });
+  __syncthreads();
+  if (k_begin >= k_end && p.splits > 1) return;  // the join does not look at this part
+  if (wave == 0 && hh == 0 && r < rows) {
+    if (p.splits == 1) {
+      if (p.lse) p.lse[(int64_t)w.bn * p.M + row] = mj + __log2f(lj);
+      sml[0][0][r] = k_begin < k_end ? 1.f / lj : 0.f;
+    } else {
+      const int64_t at = ((int64_t)w.split * p.B * p.N + w.bn) * p.M + row;
+      p.part_ml[2 * at] = mj;
+      p.part_ml[2 * at + 1] = lj;
+    }
+  }
+  __syncthreads();
+  const int quads = p.D >> 2;
+  for (int c = threadIdx.x; c < rows * quads; c += kThreads) {
+    const int i = c / quads, col = (c - i * quads) * 4;
+    float4 a = *reinterpret_cast<const float4*>(&sm.o[0][i][col]);
+#pragma unroll
+    for (int v = 1; v < 4; ++v) {
+      const float4 b = *reinterpret_cast<const float4*>(&sm.o[v][i][col]);
+      a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
+    }
+    if (p.splits == 1) {
+      const float inv = sml[0][0][i];
+      u16v<4> out;
+      out[0] = E::put(a.x * inv), out[1] = E::put(a.y * inv), out[2] = E::put(a.z * inv), out[3] = E::put(a.w * inv);
+      *reinterpret_cast<u16v<4>*>(p.out + p.dense_at(m0 + i, w.b, w.n) + col) = out;
+    } else {
+      const int64_t at = ((int64_t)w.split * p.B * p.N + w.bn) * p.M + m0 + i;
+      *reinterpret_cast<float4*>(p.part + at * p.D + col) = a;
+    }
+  }
+}
+
+// Joins the parts of split rows: four columns of a row per thread.
+template <typename E>
+__global__ void __launch_bounds__(kThreads) cross_join_kernel(CrossParams p, int64_t items) {
+  const int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (u >= items) return;
+  const int quads = p.D >> 2;
+  const int64_t stat = u / quads;  // bn M + row
+  const int col = (int)(u - stat * quads) * 4;
+  const int bn = (int)(stat / p.M), row = (int)(stat - (int64_t)bn * p.M);
+  const int b = bn / p.N, n = bn - b * p.N;
+  const int len = p.length(b);
+  const int parts = (len + p.per_split - 1) / p.per_split;
+  const int64_t step = (int64_t)p.B * p.N * p.M;
+  float m = -INFINITY;
+  for (int s = 0; s < parts; ++s) m = fmaxf(m, p.part_ml[2 * (s * step + stat)]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < parts; ++s) {
+    const int64_t at = s * step + stat;
+    const float e = exp2_fast(p.part_ml[2 * at] - base);
+    const float4 v = *reinterpret_cast<const float4*>(p.part + at * p.D + col);
+    l += p.part_ml[2 * at + 1] * e;
+    a.x += v.x * e, a.y += v.y * e, a.z += v.z * e, a.w += v.w * e;
+  }
+  const float inv = len > 0 ? 1.f / l : 0.f;
+  u16v<4> out;
+  out[0] = E::put(a.x * inv), out[1] = E::put(a.y * inv), out[2] = E::put(a.z * inv), out[3] = E::put(a.w * inv);
+  *reinterpret_cast<u16v<4>*>(p.out + p.dense_at(row, b, n) + col) = out;
+  if (p.lse && col == 0) p.lse[stat] = m + __log2f(l);
+}
+
+// ------------------------------------------------------------------------------ backward
+
+template <typename E, int DP>
+__global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
+  typedef Tile<DP> L;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2][2][kKeys * L::RB];  // [buffer][K | V]
+  const Place w(p);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 31, hh = lane >> 5;
+  const int m0 = w.block * kRows + wave * 32, row = m0 + r;
+  const bool some = m0 < p.M, mine = row < p.M;
+  const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
+  const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh;
+  const int64_t dense = mine ? p.dense_at(row, w.b, w.n) : 0, stat = (int64_t)w.bn * p.M + row;
+  u16x8 qf[L::KS], df[L::KS];
+  load_row<DP>(df, mine ? p.dout + dense : nullptr, hh, p.D);
+  float delta = 0.f, lse = INFINITY;
+  {
+    load_row<DP>(qf, mine ? p.o + dense : nullptr, hh, p.D);
+#pragma unroll
+    for (int s = 0; s < L::KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += E::get(df[s][j]) * E::get(qf[s][j]);
+    delta += __shfl_xor(delta, 32, 64);
+    if (mine) {
+      lse = p.lse[stat];
+      if (hh == 0 && w.split == 0) p.delta[stat] = delta;
+    }
+  }
+  load_row<DP>(qf, mine ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
+  f32x16 dq[L::NB];
+#pragma unroll
+  for (int nb = 0; nb < L::NB; ++nb) dq[nb] = zero16();
+  Stage<DP, kKeys> stage;
+  auto load = [&](int k0) {
+    stage.load([&](int which, int i) { return k0 + i < k_end ? kbase + (int64_t)(k0 + i) * p.kt + which * p.ks : nullptr; }, p.D);
+  };
+  if (k_begin < k_end) {
+    load(k_begin);
+    stage.store(smem[0][0], smem[0][1]);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = k_begin; k0 < k_end; k0 += kKeys, buf ^= 1) {
+    const bool more = k0 + kKeys < k_end;
+    if (more) load(k0 + kKeys);
+    const unsigned char *Ks = smem[buf][0], *Vs = smem[buf][1];
+    if (some) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int st = 0; st < L::KS; ++st) {
+          s = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s);
+          dp = mfma<E>(L::row8(Vs, kb * 32 + r, 2 * st + hh), df[st], dp);
+        }
+        const bool edge = k0 + kb * 32 + 32 > k_end;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse));
+          if (edge && k0 + kb * 32 + acc_row(i, hh) >= k_end) pv = 0.f;
+          dp[i] = pv * (dp[i] - delta);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const u16x8 db = to_operand<E>(dp, ks);
+#pragma unroll
+          for (int nb = 0; nb < L::NB; ++nb) dq[nb] = mfma<E>(L::tr8(Ks, kb * 32 + 16 * ks, nb * 32, lane), db, dq[nb]);
+        }
+      }
+    }
+    if (more) stage.store(smem[buf ^ 1][0], smem[buf ^ 1][1]);
+    __syncthreads();
+  }
+  if (!mine) return;
+  if (p.splits == 1) {
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4<E>(p.out + dense + col, dq[nb], i, p.scale); });
+  } else {
+    float* at = p.part + w.split * p.out_numel + dense;
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4f(at + col, dq[nb], i, p.scale); });
+  }
+}
+
+// 128 keys, key on the lane; row tiles of RT through LDS.
+template <typename E, int DP, int RT>
+__global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) cross_dkv_kernel(CrossParams p) {
+  typedef Tile<DP> L;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2][2][RT * L::RB];  // [buffer][Q | dO]
+  __shared__ __attribute__((aligned(16))) float sstat[2][2][RT];                 // [buffer][lse | delta]
+  const Place w(p);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 31, hh = lane >> 5;
+  const int kw = w.block * kRows + wave * 32, key = kw + r;
+  const int len = p.length(w.b);
+  const bool some = kw < len;
+  // a block of keys behind the last state has no work but its zeros
+  const int r_begin = w.split * p.per_split;
+  const int r_end = w.block * kRows < len ? min(p.M, r_begin + p.per_split) : r_begin;
+  const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh + (int64_t)key * p.kt;
+  u16x8 kf[L::KS], vf[L::KS];
+  load_row<DP>(kf, key < len ? kbase : nullptr, hh, p.D);
+  load_row<DP>(vf, key < len ? kbase + p.ks : nullptr, hh, p.D);
+  f32x16 dk[L::NB], dv[L::NB];
+#pragma unroll
+  for (int nb = 0; nb < L::NB; ++nb) dk[nb] = dv[nb] = zero16();
+  Stage<DP, RT> stage;
+  float sv = 0.f;
+  auto load = [&](int r0) {
+    stage.load(
+        [&](int which, int i) -> const u16* {
+          if (r0 + i >= r_end) return nullptr;
+          return which ? p.dout + p.dense_at(r0 + i, w.b, w.n) : p.q + p.row_at(r0 + i, w.b, w.n, p.qb, p.qt, p.qh);
+        },
+        p.D);
+    if (threadIdx.x < 2 * RT) {  // rows outside: P = 2^(0 - inf) = 0
+      const int i = threadIdx.x % RT;
+      const bool is_lse = threadIdx.x < RT;
+      sv = is_lse ? INFINITY : 0.f;
+      if (r0 + i < r_end) sv = (is_lse ? p.lse : p.delta)[(int64_t)w.bn * p.M + r0 + i];
+    }
+  };
+  auto store = [&](int buf) {
+    stage.store(smem[buf][0], smem[buf][1]);
+    if (threadIdx.x < 2 * RT) sstat[buf][threadIdx.x / RT][threadIdx.x % RT] = sv;
+  };
+  if (r_begin < r_end) {
+    load(r_begin);
+    store(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int r0 = r_begin; r0 < r_end; r0 += RT, buf ^= 1) {
+    const bool more = r0 + RT < r_end;
+    if (more) load(r0 + RT);
+    const unsigned char *Qs = smem[buf][0], *Ds = smem[buf][1];
+    if (some) {
+#pragma unroll
+      for (int qs = 0; qs < RT / 32; ++qs) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int st = 0; st < L::KS; ++st) {
+          s = mfma<E>(L::row8(Qs, qs * 32 + r, 2 * st + hh), kf[st], s);
+          dp = mfma<E>(L::row8(Ds, qs * 32 + r, 2 * st + hh), vf[st], dp);
+        }
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const int qi = qs * 32 + 8 * g4 + 4 * hh;
+          const float4 l4 = *reinterpret_cast<const float4*>(&sstat[buf][0][qi]);
+          const float4 d4 = *reinterpret_cast<const float4*>(&sstat[buf][1][qi]);
+          const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * g4 + j;
+            const float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -ls[j]));
+            s[i] = pv;
+            dp[i] = pv * (dp[i] - dl[j]);
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const u16x8 pb = to_operand<E>(s, ks), db = to_operand<E>(dp, ks);
+#pragma unroll
+          for (int nb = 0; nb < L::NB; ++nb) {
+            dv[nb] = mfma<E>(L::tr8(Ds, qs * 32 + 16 * ks, nb * 32, lane), pb, dv[nb]);
+            dk[nb] = mfma<E>(L::tr8(Qs, qs * 32 + 16 * ks, nb * 32, lane), db, dk[nb]);
+          }
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+  if (key >= p.Tk) return;
+  // a lane whose key lies behind the last state has been computing with zeros for its key: its columns are not used
+  const bool live = key < len;
+  const int64_t at = (((int64_t)w.b * p.Tk + key) * 2 * p.N + w.n) * p.D, to_v = (int64_t)p.N * p.D;
+  if (!live) {
+#pragma unroll
+    for (int nb = 0; nb < L::NB; ++nb) dk[nb] = dv[nb] = zero16();
+  }
+  if (p.splits == 1) {
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) {
+      put4<E>(p.dkv + at + col, dk[nb], i, p.scale);
+      put4<E>(p.dkv + at + to_v + col, dv[nb], i, 1.f);
+    });
+  } else {
+    float* to = p.part + w.split * p.dkv_numel + at;
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) {
+      put4f(to + col, dk[nb], i, p.scale);
+      put4f(to + to_v + col, dv[nb], i, 1.f);
+    });
+  }
+}
+
+// out[i] = sum over parts of part[s][i], in their order; numel is a multiple of 8
+template <typename E>
+__global__ void __launch_bounds__(kThreads) cross_sum_kernel(const float* __restrict__ part, u16* __restrict__ out,
+                                                             int64_t numel, int parts) {
+  const int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8;
+  if (at >= numel) return;
+  float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < parts; ++s) {
+    const auto v = load_pack<float, 8>(part + s * numel + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] += v.v[j];
+  }
+  u16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = E::put(a[j]);
+  *reinterpret_cast<u16x8*>(out + at) = o;
+}
+
+// ------------------------------------------------------------------------------ host side
+
+constexpr int kWanted = 512;  // workgroups that fill the chip: two on each of 256 CUs
+
+int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Splits an axis of `len` into parts of whole tiles so that `have` workgroups become about kWanted.
+void split_axis(CrossParams& p, int64_t have, int len, int tile, int least) {
+  int splits = (int)std::max<int64_t>(1, std::min<int64_t>(kWanted / std::max<int64_t>(1, have), up(len, least)));
+  p.per_split = std::max(tile, up(up(len, splits), tile) * tile);
+  p.splits = std::max(1, up(len, p.per_split));
+}
+
+unsigned grid_of(const CrossParams& p) {
+  const int64_t g = (int64_t)p.blocks * p.splits * p.B * p.N;
+  TORCH_CHECK(g < (1ll << 31), "cross_attention: too many workgroups");
+  return (unsigned)g;
+}
+
+template <typename F>
+void by_type_and_width(const CrossParams& p, at::ScalarType t, F&& f) {
+  using std::integral_constant;
+  auto width = [&](auto e) {
+    if (p.D <= 64) f(e, integral_constant<int, 64>{});
+    else if (p.D <= 96) f(e, integral_constant<int, 96>{});
+    else f(e, integral_constant<int, 128>{});
+  };
+  t == at::kBFloat16 ? width(BF16{}) : width(FP16{});
+}
+
+typedef c10::optional<at::Tensor> OptTensor;
+
+CrossParams cross_params(const at::Tensor& q, const at::Tensor& kv, const OptTensor& lengths, double scale) {
+  CrossParams p{};
+  p.q = (const u16*)q.data_ptr();
+  p.kv = (const u16*)kv.data_ptr();
+  p.qb = q.stride(0), p.qt = q.stride(1), p.qh = q.stride(2);
+  p.kb = kv.stride(0), p.kt = kv.stride(1), p.ks = kv.stride(2), p.kh = kv.stride(3);
+  p.B = (int)q.size(0), p.Tq = (int)q.size(1), p.Tk = (int)kv.size(1), p.N = (int)kv.size(3), p.D = (int)q.size(3);
+  p.G = (int)(q.size(2) / kv.size(3));
+  p.M = p.G * p.Tq;
+  p.by_G = FastDiv((unsigned)p.G);
+  if (lengths) {
+    p.lengths = lengths->data_ptr();
+    p.len64 = lengths->scalar_type() == at::kLong;
+  }
+  p.scale = (float)scale;
+  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.out_numel = q.numel();
+  p.dkv_numel = kv.numel();
+  p.splits = 1;
+  return p;
+}
+
+// q and kv are laid out for the kernels; lse only where a backward pass will want it
+std::vector<at::Tensor> cross_fwd(const at::Tensor& q, const at::Tensor& kv, const OptTensor& lengths, double scale,
+                                  bool with_lse) {
+  c10::DeviceGuard guard(q.device());
+  CrossParams p = cross_params(q, kv, lengths, scale);
+  auto out = at::empty(q.sizes(), q.options());
+  at::Tensor lse, part, ml;
+  const auto f32 = q.options().dtype(at::kFloat);
+  if (with_lse) lse = at::empty({p.B, p.N, p.M}, f32);
+  if (out.numel() == 0) return {out, lse};
+  if (p.Tk == 0) {
+    out.zero_();
+    return {out, lse};
+  }
+  p.out = (u16*)out.data_ptr();
+  p.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+  const bool few = p.M <= 32;
+  p.blocks = up(p.M, few ? 32 : kRows);
+  split_axis(p, (int64_t)p.blocks * p.B * p.N, p.Tk, few ? 128 : kKeys, 256);
+  if (p.splits > 1) {
+    part = at::empty({p.splits, (int64_t)p.B * p.N * p.M * p.D}, f32);
+    ml = at::empty({p.splits, (int64_t)p.B * p.N * p.M, 2}, f32);
+    p.part = part.data_ptr<float>();
+    p.part_ml = ml.data_ptr<float>();
+  }
+  const unsigned grid = grid_of(p);
+  by_type_and_width(p, q.scalar_type(), [&](auto e, auto dp) {
+    typedef decltype(e) E;
+    if (few)
+      hipLaunchKernelGGL((cross_few_kernel<E, dp>), dim3(grid), dim3(kThreads), 0, stream(), p);
+    else
+      hipLaunchKernelGGL((cross_fwd_kernel<E, dp>), dim3(grid), dim3(kThreads), 0, stream(), p);
+    LAUNCH_CHECK();
+    if (p.splits > 1) {
+      const int64_t items = (int64_t)p.B * p.N * p.M * (p.D / 4);
+      hipLaunchKernelGGL((cross_join_kernel<E>), dim3((unsigned)up(items, kThreads)), dim3(kThreads), 0, stream(), p, items);
+      LAUNCH_CHECK();
+    }
+  });
+  return {out, lse};
+}
+
+std::vector<at::Tensor> cross_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& kv, const at::Tensor& out,
+                                  const at::Tensor& lse, const OptTensor& lengths, double scale) {
+  c10::DeviceGuard guard(q.device());
+  CrossParams p = cross_params(q, kv, lengths, scale);
+  auto dq = at::empty(q.sizes(), q.options()), dkv = at::empty(kv.sizes(), kv.options());
+  if (q.numel() == 0 || kv.numel() == 0) return {dq.zero_(), dkv.zero_()};
+  const auto f32 = q.options().dtype(at::kFloat);
+  auto delta = at::empty({p.B, p.N, p.M}, f32);
+  p.o = (const u16*)out.data_ptr();
+  p.dout = (const u16*)dout.data_ptr();
+  p.out = (u16*)dq.data_ptr();
+  p.dkv = (u16*)dkv.data_ptr();
+  p.lse = lse.data_ptr<float>();
+  p.delta = delta.data_ptr<float>();
+  by_type_and_width(p, q.scalar_type(), [&](auto e, auto dp) {
+    typedef decltype(e) E;
+    constexpr int RT = dp <= 64 ? 64 : 32;
+    auto sum = [&](const at::Tensor& part, at::Tensor& to) {
+      const int64_t n = to.numel();
+      hipLaunchKernelGGL((cross_sum_kernel<E>), dim3((unsigned)up(n, 8 * kThreads)), dim3(kThreads), 0, stream(),
+                         part.data_ptr<float>(), (u16*)to.data_ptr(), n, p.splits);
+      LAUNCH_CHECK();
+    };
+    at::Tensor part;
+    p.blocks = up(p.M, kRows);
+    split_axis(p, (int64_t)p.blocks * p.B * p.N, p.Tk, kKeys, 256);
+    if (p.splits > 1) {
+      part = at::empty({p.splits, p.out_numel}, f32);
+      p.part = part.data_ptr<float>();
+    }
+    hipLaunchKernelGGL((cross_dq_kernel<E, dp>), dim3(grid_of(p)), dim3(kThreads), 0, stream(), p);
+    LAUNCH_CHECK();
+    if (p.splits > 1) sum(part, dq);
+    p.blocks = up(p.Tk, kRows);
+    split_axis(p, (int64_t)p.blocks * p.B * p.N, p.M, RT, 128);
+    if (p.splits > 1) {
+      part = at::empty({p.splits, p.dkv_numel}, f32);
+      p.part = part.data_ptr<float>();
+    }
+    hipLaunchKernelGGL((cross_dkv_kernel<E, dp, RT>), dim3(grid_of(p)), dim3(kThreads), 0, stream(), p);
+    LAUNCH_CHECK();
+    if (p.splits > 1) sum(part, dkv);
+  });
+  return {dq, dkv};
+}
+
+// Rows of whole 16-byte chunks at 16-byte addresses, or a copy that has them.
+at::Tensor chunked(const at::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok &= t.size(i) == 1 || t.stride(i) % 8 == 0;
+  if (ok) return t;
+  auto c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct CrossFn : public torch::autograd::Function<CrossFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& kv, const OptTensor& lengths,
+                            double scale) {
+    auto qc = chunked(q), kc = chunked(kv);
+    auto r = cross_fwd(qc, kc, lengths, scale, true);
+    ctx->save_for_backward({qc, kc, r[0], r[1], lengths ? *lengths : at::Tensor()});
+    ctx->saved_data["scale"] = scale;
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "cross_attention: second derivatives are not implemented");
+    auto s = ctx->get_saved_variables();
+    OptTensor lengths;
+    if (s[4].defined()) lengths = s[4];
+    auto g = grads[0].contiguous();
+    if (reinterpret_cast<uintptr_t>(g.data_ptr()) % 16) g = g.clone();
+    auto d = cross_bwd(g, s[0], s[1], s[2], s[3], lengths, ctx->saved_data["scale"].toDouble());
+    return {d[0], d[1], at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& kv, const OptTensor& lengths, double scale) {
+  const char* op = "cross_attention: ";
+  TORCH_CHECK(q.is_cuda() && kv.device() == q.device(), op, "q and kv must be on one GPU");
+  TORCH_CHECK(q.scalar_type() == kv.scalar_type() && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf), op,
+              "q and kv must both be bfloat16 or float16");
+  TORCH_CHECK(q.dim() == 4 && kv.dim() == 5 && kv.size(2) == 2, op, "q must be [B, Tq, H, D] and kv [B, Tk, 2, N, D]");
+  TORCH_CHECK(q.size(0) == kv.size(0) && q.size(3) == kv.size(4), op, "q and kv must agree in B and D");
+  TORCH_CHECK(q.size(3) % 8 == 0 && q.size(3) >= 8 && q.size(3) <= 128, op, "D must be a multiple of 8 up to 128");
+  TORCH_CHECK(kv.size(3) > 0 && q.size(2) > 0 && q.size(2) % kv.size(3) == 0, op, "N must divide H");
+  TORCH_CHECK(q.size(1) * q.size(2) < (1ll << 31) - kRows && kv.size(1) < (1ll << 31) - kRows && q.size(0) < (1ll << 31), op,
+              "fewer than 2^31 rows and states wanted");
+  TORCH_CHECK(std::isfinite(scale) && scale > 0.0, op, "scale must be positive");
+  OptTensor len;
+  if (lengths) {
+    TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == q.size(0) && lengths->device() == q.device() &&
+                    (lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong),
+                op, "lengths must be int32 or int64 [B] on the device of q");
+    len = lengths->contiguous();
+  }
+  if (at::GradMode::is_enabled() && (q.requires_grad() || kv.requires_grad())) return CrossFn::apply(q, kv, len, scale);
+  return cross_fwd(chunked(q), chunked(kv), len, scale, false)[0];
+}
+
+}  // namespace
+
+void register_cross_attention(pybind11::module_& m) {
+  m.def("cross_attention", &cross_attention, "attention of q [B, Tq, H, D] over packed kv [B, Tk, 2, N, D]");
+}

@@ -7,6 +7,7 @@
     loss = fused.cross_entropy(logits, t) # mean CE on bf16 logits [N, V]
     qkv = fused.rotary_qkv(qkv, positions, freqs)     # q and k turned by their positions
     x, h = fused.dropout_add_rms_norm(x, delta, norm.weight, p, seed)  # no mask is stored
+    o = fused.cross_attention(q, kv, lengths)         # over an encoder's states of another length
 
 On a GPU the HIP kernels are mandatory: if the in-tree extension is missing or broken the
 first call raises (no silent eager fallback). On CPU tensors (tests, CPU smoke runs) the plain
@@ -182,6 +183,54 @@ def attention(qkv: torch.Tensor, causal: bool = True, scale: float | None = None
     o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=causal,
                                        scale=scale)
     return o.transpose(1, 2)
+
+
+def cross_attention(q: torch.Tensor, kv: torch.Tensor, lengths: torch.Tensor | None = None,
+                    scale: float | None = None) -> torch.Tensor:
+    """Attention of queries q [B, Tq, H, D] over another sequence's states, kv [B, Tk, 2, N, D] (its packed
+    key and value projection; N divides H, and H / N neighbouring heads share a key head) -> [B, Tq, H, D].
+
+    lengths: int32 or int64 [B], how many of the Tk states each sequence has (None: all; values outside
+    0..Tk are taken as the nearest). States behind them are never read, whatever they hold, and their
+    gradients are 0; a sequence of no states gives 0. Any strides; Tq and Tk of any length, one query token
+    included (serving). bfloat16 and float16 run the gfx950 kernels on a GPU (MFMA, forward and backward),
+    with D a multiple of 8 up to 128; float32 and float64 are computed in PyTorch ops."""
+    if q.dim() != 4 or kv.dim() != 5 or kv.shape[2] != 2:
+        raise ValueError("cross_attention: q must be [B, Tq, H, D] and kv [B, Tk, 2, N, D]")
+    b, _, h, d = q.shape
+    if kv.shape[0] != b or kv.shape[4] != d or q.dtype != kv.dtype or q.device != kv.device:
+        raise ValueError("cross_attention: q and kv must agree in B, D, type and device")
+    if kv.shape[3] == 0 or h == 0 or h % kv.shape[3]:
+        raise ValueError("cross_attention: N must divide H")
+    if lengths is not None and (lengths.shape != (b,) or lengths.dtype not in (torch.int32, torch.int64)
+                                or lengths.device != q.device):
+        raise ValueError("cross_attention: lengths must be int32 or int64 [B] on the device of q")
+    if scale is None:
+        scale = d ** -0.5
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("cross_attention: scale must be positive")
+    if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16):
+        return ext().cross_attention(q, kv, lengths, float(scale))
+    return _cross_attention_eager(q, kv, lengths, scale)
+
+
+def _cross_attention_eager(q, kv, lengths, scale):
+    b, tq, h, d = q.shape
+    tk, n = kv.shape[1], kv.shape[3]
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    kv = kv.to(wide)
+    if lengths is not None:
+        off = torch.arange(tk, device=q.device) >= lengths[:, None]
+        kv = kv.masked_fill(off[:, :, None, None, None], 0.0)
+    k, v = kv.permute(2, 0, 3, 1, 4)  # [B, N, Tk, D]
+    rows = q.to(wide).reshape(b, tq, n, h // n, d).permute(0, 2, 3, 1, 4).reshape(b, n, -1, d)
+    s = rows @ k.transpose(2, 3).contiguous() * scale
+    if lengths is not None:
+        s = s.masked_fill(off[:, None, None], -math.inf)
+        p = torch.softmax(s, -1).masked_fill((lengths <= 0)[:, None, None, None], 0.0)
+    else:
+        p = torch.softmax(s, -1)
+    return (p @ v.contiguous()).view(b, n, h // n, tq, d).permute(0, 3, 1, 2, 4).reshape(b, tq, h, d).to(q.dtype)
 
 
 # ------------------------------------------------------------------------------ rotary positions

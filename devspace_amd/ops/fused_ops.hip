@@ -27,6 +27,7 @@
 
 void register_rotary(pybind11::module_& m);
 void register_dropout(pybind11::module_& m);
+void register_cross_attention(pybind11::module_& m);
 
 namespace {
 
@@ -1557,4 +1558,5 @@ PYBIND11_MODULE(_fused_ops, m) {
   m.def("ce_bwd", &ce_bwd);
   register_rotary(m);
   register_dropout(m);
+  register_cross_attention(m);
 }

@@ -31,6 +31,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRows = 128;  // query rows (forward, dQ) or keys (dK, dV) of a workgroup: 32 per wave
 constexpr int kKeys = 64;   // keys of an LDS tile
+constexpr int kWanted = 512;  // workgroups that fill the chip: two on each of 256 CUs
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -38,6 +39,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
+typedef __attribute__((address_space(3))) void lds_void;
 
 template <typename E>
 __device__ __forceinline__ f32x16 mfma(const u16x8& a, const u16x8& b, const f32x16& c) {
@@ -56,6 +58,7 @@ struct Tile {
   static constexpr int CH = DP / 8;   // chunks of a row
   static constexpr int KS = DP / 16;  // steps of a product over the columns
   static constexpr int NB = DP / 32;  // blocks of 32 columns
+  static constexpr int BUFS = DP <= 64 ? 3 : 2;  // tiles in LDS, with two workgroups on a CU
   __device__ static __forceinline__ int off(int row, int chunk) {
     if constexpr (RB == 128) return row * 128 + ((chunk ^ ((row >> 1) & 7) ^ ((row & 2) << 1)) << 4);
     else return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
@@ -123,7 +126,7 @@ struct CrossParams {
   __device__ __forceinline__ int length(int b) const {
     if (!lengths) return Tk;
     const int64_t n = len64 ? static_cast<const int64_t*>(lengths)[b] : (int64_t)static_cast<const int*>(lengths)[b];
-    return (int)(n < 0 ? 0 : n > Tk ? Tk : n);
+    return __builtin_amdgcn_readfirstlane((int)(n < 0 ? 0 : n > Tk ? Tk : n));
   }
   // offset of row m of key head n in [B, Tq, H, D] with these strides
   __device__ __forceinline__ int64_t row_at(int m, int b, int n, int64_t sb, int64_t st, int64_t sh) const {
@@ -154,35 +157,68 @@ struct Place {
   }
 };
 
-// 256 threads carry one tile of ROWS rows of two tensors through registers into LDS; rows and columns
-// outside are 0 and never read.
+// One wave's share of copying tiles of ROWS rows of two tensors (waves 0 and 1 the first, 2 and 3 the second)
+// straight into LDS: buffer loads that write there without passing registers, 64 lanes x 16 bytes, a few whole
+// rows each. The swizzle is applied to the source: lane l fills the l-th 16 bytes and fetches the chunk that
+// belongs there. Rows and columns outside get an offset beyond the buffer, which reads as 0.
+constexpr unsigned kOutside = 0x80000000u;
+
+// BYTES (4 or 16) per lane from `base` plus this lane's offset to `lds` plus BYTES times the lane
+template <int BYTES>
+__device__ __forceinline__ void to_lds(const void* base, void* lds, unsigned offset) {
+#ifdef __HIP_DEVICE_COMPILE__  // the buffer's type is the device's
+  __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, kOutside - 1, 0x00020000);
+  static_assert(BYTES == 16 || BYTES == 4, "sizes used here");
+  if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(lds_u8*)lds, 16, offset, 0, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(lds_u8*)lds, 4, offset, 0, 0, 0);
+#endif
+}
+
 template <int DP, int ROWS>
-struct Stage {
+struct Dma {
   typedef Tile<DP> L;
-  static constexpr int kEach = ROWS * L::CH;
-  static constexpr int kPer = 2 * kEach / kThreads;
-  static_assert(2 * kEach % kThreads == 0, "whole chunks per thread");
-  u16x8 r[kPer];
+  static constexpr int kPer = 2 * ROWS * L::RB / (4 * 1024);  // loads of a wave
+  static constexpr int kRowsEach = 1024 / L::RB;
+  static constexpr int kSlots = L::RB / 16;
+  unsigned at[kPer];  // byte offset of this lane's chunk from the tile's first row
+  int first;          // this lane's row in the wave's first load
+  int piece;          // where the wave's part of a tensor's tile begins, bytes
+
+  __device__ static __forceinline__ bool second(int wave) { return wave >= 2; }
+
+  // offset(row): byte offset of a row of the tile
   template <typename F>
-  __device__ __forceinline__ void load(F&& at, int D) {  // at(which, row): the row's first element, or null
+  __device__ __forceinline__ void init(int wave, int lane, int D, F&& offset) {
+    first = (wave & 1) * (ROWS / 2) + lane / kSlots;
+    piece = (wave & 1) * (ROWS / 2) * L::RB;
+    place(lane, D, offset);
+  }
+  template <typename F>
+  __device__ __forceinline__ void place(int lane, int D, F&& offset) {
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
-      const int c = threadIdx.x + kThreads * u;
-      const int which = c >= kEach, cc = c - which * kEach;
-      const int row = cc / L::CH, ch = cc % L::CH;
-      const u16* src = ch * 8 < D ? at(which, row) : nullptr;
-      r[u] = src ? *reinterpret_cast<const u16x8*>(src + ch * 8) : zero8();
+      const int row = first + u * kRowsEach;
+      const int chunk = (L::off(row, lane % kSlots) - row * L::RB) >> 4;
+      at[u] = chunk * 8 < D ? offset(row) + chunk * 16 : kOutside;
     }
   }
-  __device__ __forceinline__ void store(unsigned char* ta, unsigned char* tb) {
+  // rows [0, valid) of the tile that begins at `base`; valid <= 0 fills the tile with zeros
+  __device__ __forceinline__ void go(const u16* base, unsigned char* tile, int valid) const {
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const int c = threadIdx.x + kThreads * u;
-      const int which = c >= kEach, cc = c - which * kEach;
-      *reinterpret_cast<u16x8*>((which ? tb : ta) + L::off(cc / L::CH, cc % L::CH)) = r[u];
-    }
+    for (int u = 0; u < kPer; ++u)
+      to_lds<16>(base, tile + piece + u * 1024, first + u * kRowsEach < valid ? at[u] : kOutside);
   }
 };
+
+// All but the wave's last N loads have arrived, its LDS reads are done, and the other waves are as far.
+template <int N>
+__device__ __forceinline__ void wait_all_but() {
+  static_assert(N < 64, "the counter has six bits");
+  if constexpr (N == 0)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
 // this lane's half of a row as KS operands (columns 16 s + 8 hh ..); null: zeros
 template <int DP>
@@ -242,67 +278,116 @@ __device__ __forceinline__ void put4f(float* at, const f32x16& a, int i, float b
   *reinterpret_cast<float4*>(at) = make_float4(a[i] * by, a[i + 1] * by, a[i + 2] * by, a[i + 3] * by);
 }
 
+// Runs step(tile, position) over positions begin, begin + STEP, ... < end, with the tiles of the next BUFS - 1
+// positions on their way: issue(tile, position) starts a tile's PER loads of this wave (positions past the end
+// too, so that the number of loads in flight does not depend on the position). A position's loads are waited
+// for, then the barrier says that all waves have waited, and have left the tile that is filled next. The tiles
+// are separate arrays, so that the compiler knows that reads of one need not wait for loads into another.
+template <int PER, int STEP, typename T, typename I, typename S>
+__device__ __forceinline__ void pipeline(T& a, T& b, int begin, int end, I&& issue, S&& step) {
+  issue(a, begin);
+  for (int at = begin;;) {
+    wait_all_but<0>();
+    issue(b, at + STEP);
+    step(a, at);
+    if ((at += STEP) >= end) break;
+    wait_all_but<0>();
+    issue(a, at + STEP);
+    step(b, at);
+    if ((at += STEP) >= end) break;
+  }
+  wait_all_but<0>();
+}
+template <int PER, int STEP, typename T, typename I, typename S>
+__device__ __forceinline__ void pipeline(T& a, T& b, T& c, int begin, int end, I&& issue, S&& step) {
+  issue(a, begin);
+  issue(b, begin + STEP);
+  for (int at = begin;;) {
+    wait_all_but<PER>();
+    issue(c, at + 2 * STEP);
+    step(a, at);
+    if ((at += STEP) >= end) break;
+    wait_all_but<PER>();
+    issue(a, at + 2 * STEP);
+    step(b, at);
+    if ((at += STEP) >= end) break;
+    wait_all_but<PER>();
+    issue(b, at + 2 * STEP);
+    step(c, at);
+    if ((at += STEP) >= end) break;
+  }
+  wait_all_but<0>();
+}
+
+template <int DP>
+using KeyTile = unsigned char[2][kKeys * Tile<DP>::RB];  // K | V
+#define KEY_TILES(DP) __shared__ __attribute__((aligned(16))) KeyTile<DP> tile0, tile1, tile2
+
+// step(K tile, V tile, first key) over the keys [begin, end) of one key head
+template <int DP, typename S>
+__device__ __forceinline__ void key_loop(KeyTile<DP>& tile0, KeyTile<DP>& tile1, KeyTile<DP>& tile2, const CrossParams& p,
+                                         const Place& w, int wave, int lane, int begin, int end, S&& step) {
+  typedef Tile<DP> L;
+  typedef Dma<DP, kKeys> Copy;
+  typedef KeyTile<DP> Pair;
+  if (begin >= end) return;
+  Copy copy;
+  copy.init(wave, lane, p.D, [&](int row) { return (unsigned)(row * (int)p.kt * 2); });
+  const bool second = Copy::second(wave);
+  const u16* base = p.kv + w.b * p.kb + w.n * p.kh + (second ? p.ks : 0);
+  auto issue = [&](Pair& t, int k0) { copy.go(base + (k0 < end ? k0 : 0) * p.kt, t[second], end - k0); };
+  auto use = [&](const Pair& t, int k0) { step(t[0], t[1], k0); };
+  if constexpr (L::BUFS == 3) pipeline<Copy::kPer, kKeys>(tile0, tile1, tile2, begin, end, issue, use);
+  else pipeline<Copy::kPer, kKeys>(tile0, tile1, begin, end, issue, use);
+}
+
 // ------------------------------------------------------------------------------ forward
 
 template <typename E, int DP>
 __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
   typedef Tile<DP> L;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2][2][kKeys * L::RB];  // [buffer][K | V]
+  KEY_TILES(DP);
   const Place w(p);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, hh = lane >> 5;
   const int m0 = w.block * kRows + wave * 32, row = m0 + r;
   const bool some = m0 < p.M;  // the wave has rows at all
   const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
-  const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh;
   u16x8 qf[L::KS];
   load_row<DP>(qf, row < p.M ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
   f32x16 o[L::NB];
 #pragma unroll
   for (int nb = 0; nb < L::NB; ++nb) o[nb] = zero16();
   float m = -INFINITY, l = 0.f;
-  Stage<DP, kKeys> stage;
-  auto load = [&](int k0) {
-    stage.load([&](int which, int i) { return k0 + i < k_end ? kbase + (int64_t)(k0 + i) * p.kt + which * p.ks : nullptr; }, p.D);
-  };
-  if (k_begin < k_end) {
-    load(k_begin);
-    stage.store(smem[0][0], smem[0][1]);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += kKeys, buf ^= 1) {
-    const bool more = k0 + kKeys < k_end;
-    if (more) load(k0 + kKeys);
-    const unsigned char *Ks = smem[buf][0], *Vs = smem[buf][1];
-    if (some) {
-      f32x16 s[2] = {zero16(), zero16()};
+  auto step = [&](const unsigned char* Ks, const unsigned char* Vs, int k0) {
+    if (!some) return;
+    f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
-      for (int st = 0; st < L::KS; ++st)
+    for (int st = 0; st < L::KS; ++st)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) s[kb] = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s[kb]);
-      if (k0 + kKeys > k_end) {
+      for (int kb = 0; kb < 2; ++kb) s[kb] = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s[kb]);
+    if (k0 + kKeys > k_end) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (k0 + kb * 32 + acc_row(i, hh) >= k_end) s[kb][i] = -INFINITY;
-      }
-      const float alpha = soften<2>(s, m, l, p.scale_log2);
+        for (int i = 0; i < 16; ++i)
+          if (k0 + kb * 32 + acc_row(i, hh) >= k_end) s[kb][i] = -INFINITY;
+    }
+    const float alpha = soften<2>(s, m, l, p.scale_log2);
+    if (__any(alpha != 1.f)) {  // some row of the wave has a new maximum
 #pragma unroll
       for (int nb = 0; nb < L::NB; ++nb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const u16x8 pb = to_operand<E>(s[ks >> 1], ks & 1);
-#pragma unroll
-        for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(L::tr8(Vs, 16 * ks, nb * 32, lane), pb, o[nb]);
-      }
     }
-    if (more) stage.store(smem[buf ^ 1][0], smem[buf ^ 1][1]);
-    __syncthreads();
-  }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const u16x8 pb = to_operand<E>(s[ks >> 1], ks & 1);
+#pragma unroll
+      for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(L::tr8(Vs, 16 * ks, nb * 32, lane), pb, o[nb]);
+    }
+  };
+  key_loop<DP>(tile0, tile1, tile2, p, w, wave, lane, k_begin, k_end, step);
   if (row >= p.M) return;
   l += __shfl_xor(l, 32, 64);
   const int64_t stat = (int64_t)w.bn * p.M + row;
@@ -445,36 +530,65 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   }
 }
 
-// Joins the parts of split rows: four columns of a row per thread.
-template <typename E>
-__global__ void __launch_bounds__(kThreads) cross_join_kernel(CrossParams p, int64_t items) {
-  const int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (u >= items) return;
-  const int quads = p.D >> 2;
-  const int64_t stat = u / quads;  // bn M + row
-  const int col = (int)(u - stat * quads) * 4;
+// Joins the parts of a split row: THREADS threads per row, 32 lanes over its columns (four each), THREADS / 32
+// groups of them over the parts, whose sums are added in LDS.
+template <typename E, int THREADS>
+__global__ void __launch_bounds__(THREADS) cross_join_kernel(CrossParams p) {
+  constexpr int kGroups = THREADS / 32;
+  __shared__ float weight[kWanted], red[2][THREADS / 64];
+  __shared__ __attribute__((aligned(16))) float acc[kGroups][128];
+  const int64_t stat = blockIdx.x;  // bn M + row
   const int bn = (int)(stat / p.M), row = (int)(stat - (int64_t)bn * p.M);
   const int b = bn / p.N, n = bn - b * p.N;
-  const int len = p.length(b);
-  const int parts = (len + p.per_split - 1) / p.per_split;
+  const int parts = (p.length(b) + p.per_split - 1) / p.per_split;
   const int64_t step = (int64_t)p.B * p.N * p.M;
+  const int wave = threadIdx.x >> 6;
   float m = -INFINITY;
-  for (int s = 0; s < parts; ++s) m = fmaxf(m, p.part_ml[2 * (s * step + stat)]);
+  for (int s = threadIdx.x; s < parts; s += THREADS) m = fmaxf(m, p.part_ml[2 * (s * step + stat)]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) red[0][wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < THREADS / 64; ++v) m = fmaxf(m, red[0][v]);
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < parts; ++s) {
+  for (int s = threadIdx.x; s < parts; s += THREADS) {
     const int64_t at = s * step + stat;
     const float e = exp2_fast(p.part_ml[2 * at] - base);
-    const float4 v = *reinterpret_cast<const float4*>(p.part + at * p.D + col);
+    weight[s] = e;
     l += p.part_ml[2 * at + 1] * e;
-    a.x += v.x * e, a.y += v.y * e, a.z += v.z * e, a.w += v.w * e;
   }
-  const float inv = len > 0 ? 1.f / l : 0.f;
+  l = wave_sum(l);
+  if ((threadIdx.x & 63) == 0) red[1][wave] = l;
+  __syncthreads();
+  l = red[1][0];
+#pragma unroll
+  for (int v = 1; v < THREADS / 64; ++v) l += red[1][v];
+  const int col = (threadIdx.x & 31) * 4, group = threadIdx.x >> 5;
+  if (col < p.D) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = group; s < parts; s += kGroups) {
+      const float4 v = *reinterpret_cast<const float4*>(p.part + (s * step + stat) * p.D + col);
+      const float e = weight[s];
+      a.x += v.x * e, a.y += v.y * e, a.z += v.z * e, a.w += v.w * e;
+    }
+    *reinterpret_cast<float4*>(&acc[group][col]) = a;
+  }
+  __syncthreads();
+  if (group > 0 || col >= p.D) return;
+  const float inv = parts > 0 ? 1.f / l : 0.f;
   u16v<4> out;
-  out[0] = E::put(a.x * inv), out[1] = E::put(a.y * inv), out[2] = E::put(a.z * inv), out[3] = E::put(a.w * inv);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float t = acc[0][col + j];
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) t += acc[g][col + j];
+    out[j] = E::put(t * inv);
+  }
   *reinterpret_cast<u16v<4>*>(p.out + p.dense_at(row, b, n) + col) = out;
-  if (p.lse && col == 0) p.lse[stat] = m + __log2f(l);
+  if (p.lse && threadIdx.x == 0) p.lse[stat] = m + __log2f(l);
 }
 
 // ------------------------------------------------------------------------------ backward
@@ -482,75 +596,87 @@ __global__ void __launch_bounds__(kThreads) cross_join_kernel(CrossParams p, int
 template <typename E, int DP>
 __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   typedef Tile<DP> L;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2][2][kKeys * L::RB];  // [buffer][K | V]
+  KEY_TILES(DP);
   const Place w(p);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, hh = lane >> 5;
   const int m0 = w.block * kRows + wave * 32, row = m0 + r;
   const bool some = m0 < p.M, mine = row < p.M;
   const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
-  const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh;
   const int64_t dense = mine ? p.dense_at(row, w.b, w.n) : 0, stat = (int64_t)w.bn * p.M + row;
   u16x8 qf[L::KS], df[L::KS];
   load_row<DP>(df, mine ? p.dout + dense : nullptr, hh, p.D);
-  float delta = 0.f, lse = INFINITY;
-  {
-    load_row<DP>(qf, mine ? p.o + dense : nullptr, hh, p.D);
+  load_row<DP>(qf, mine ? p.o + dense : nullptr, hh, p.D);
+  float delta = 0.f;
 #pragma unroll
-    for (int s = 0; s < L::KS; ++s)
+  for (int s = 0; s < L::KS; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta += E::get(df[s][j]) * E::get(qf[s][j]);
-    delta += __shfl_xor(delta, 32, 64);
-    if (mine) {
-      lse = p.lse[stat];
-      if (hh == 0 && w.split == 0) p.delta[stat] = delta;
-    }
-  }
+    for (int j = 0; j < 8; ++j) delta += E::get(df[s][j]) * E::get(qf[s][j]);
+  delta += __shfl_xor(delta, 32, 64);
+  const float lse = mine ? p.lse[stat] : INFINITY;  // rows outside: P = 2^(0 - inf) = 0
   load_row<DP>(qf, mine ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
   f32x16 dq[L::NB];
 #pragma unroll
   for (int nb = 0; nb < L::NB; ++nb) dq[nb] = zero16();
-  Stage<DP, kKeys> stage;
-  auto load = [&](int k0) {
-    stage.load([&](int which, int i) { return k0 + i < k_end ? kbase + (int64_t)(k0 + i) * p.kt + which * p.ks : nullptr; }, p.D);
+  // S and dP of 32 keys, S turned into P; keys behind the end have P = 0
+  auto scores = [&](const unsigned char* Ks, const unsigned char* Vs, int k0, int kb, f32x16& s, f32x16& dp) {
+    s = zero16();
+    dp = zero16();
+#pragma unroll
+    for (int st = 0; st < L::KS; ++st) {
+      s = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s);
+      dp = mfma<E>(L::row8(Vs, kb * 32 + r, 2 * st + hh), df[st], dp);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse));
+    if (k0 + kb * 32 + 32 > k_end) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + kb * 32 + acc_row(i, hh) >= k_end) s[i] = 0.f;
+    }
   };
-  if (k_begin < k_end) {
-    load(k_begin);
-    stage.store(smem[0][0], smem[0][1]);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += kKeys, buf ^= 1) {
-    const bool more = k0 + kKeys < k_end;
-    if (more) load(k0 + kKeys);
-    const unsigned char *Ks = smem[buf][0], *Vs = smem[buf][1];
-    if (some) {
+  auto add = [&](const unsigned char* Ks, int kb, const f32x16& s, f32x16& dp) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - delta);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const u16x8 db = to_operand<E>(dp, ks);
+#pragma unroll
+      for (int nb = 0; nb < L::NB; ++nb) dq[nb] = mfma<E>(L::tr8(Ks, kb * 32 + 16 * ks, nb * 32, lane), db, dq[nb]);
+    }
+  };
+  if (p.splits == 1 && k_end <= kKeys) {
+    // One tile holds all states. With few of them, the rounding of O weighs in dO . O, which nearly equals the
+    // dP it is taken from; here it is summed from P and dP themselves.
+    key_loop<DP>(tile0, tile1, tile2, p, w, wave, lane, k_begin, k_end, [&](const unsigned char* Ks, const unsigned char* Vs, int k0) {
+      if (!some) return;
+      f32x16 s, dp;
+      float sum = 0.f;
+#pragma unroll 1
+      for (int kb = 0; kb < 2; ++kb) {
+        scores(Ks, Vs, k0, kb, s, dp);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += s[i] * dp[i];
+      }
+      delta = sum + __shfl_xor(sum, 32, 64);
+#pragma unroll 1
+      for (int kb = 0; kb < 2; ++kb) {
+        scores(Ks, Vs, k0, kb, s, dp);
+        add(Ks, kb, s, dp);
+      }
+    });
+  } else {
+    key_loop<DP>(tile0, tile1, tile2, p, w, wave, lane, k_begin, k_end, [&](const unsigned char* Ks, const unsigned char* Vs, int k0) {
+      if (!some) return;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-        for (int st = 0; st < L::KS; ++st) {
-          s = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s);
-          dp = mfma<E>(L::row8(Vs, kb * 32 + r, 2 * st + hh), df[st], dp);
-        }
-        const bool edge = k0 + kb * 32 + 32 > k_end;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse));
-          if (edge && k0 + kb * 32 + acc_row(i, hh) >= k_end) pv = 0.f;
-          dp[i] = pv * (dp[i] - delta);
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const u16x8 db = to_operand<E>(dp, ks);
-#pragma unroll
-          for (int nb = 0; nb < L::NB; ++nb) dq[nb] = mfma<E>(L::tr8(Ks, kb * 32 + 16 * ks, nb * 32, lane), db, dq[nb]);
-        }
+        f32x16 s, dp;
+        scores(Ks, Vs, k0, kb, s, dp);
+        add(Ks, kb, s, dp);
       }
-    }
-    if (more) stage.store(smem[buf ^ 1][0], smem[buf ^ 1][1]);
-    __syncthreads();
+    });
   }
+  if (mine && hh == 0 && w.split == 0) p.delta[stat] = delta;
   if (!mine) return;
   if (p.splits == 1) {
     each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4<E>(p.out + dense + col, dq[nb], i, p.scale); });
@@ -562,12 +688,20 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
 
 // 128 keys, key on the lane; row tiles of RT through LDS.
 template <typename E, int DP, int RT>
-__global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) cross_dkv_kernel(CrossParams p) {
+__global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   typedef Tile<DP> L;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2][2][RT * L::RB];  // [buffer][Q | dO]
-  __shared__ __attribute__((aligned(16))) float sstat[2][2][RT];                 // [buffer][lse | delta]
+  typedef Dma<DP, RT> Copy;
+  constexpr int kEach = 2 * RT / 4;  // statistics that a wave fetches; its place in LDS holds 64
+  struct Rows {
+    unsigned char x[2][RT * L::RB];  // Q | dO
+    float stat[4][64];               // lse, delta: kEach of each wave
+  };
+  __shared__ __attribute__((aligned(16))) Rows tile0, tile1, tile2;
+  // with wide heads the registers do not hold V beside K, dK and dV: it is read from LDS where it is used
+  constexpr bool kVInLds = DP > 96;
+  __shared__ __attribute__((aligned(16))) unsigned char vs[kVInLds ? kRows * L::RB : 16];
   const Place w(p);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, hh = lane >> 5;
   const int kw = w.block * kRows + wave * 32, key = kw + r;
   const int len = p.length(w.b);
@@ -576,78 +710,90 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) cross_dkv_kernel(C
   const int r_begin = w.split * p.per_split;
   const int r_end = w.block * kRows < len ? min(p.M, r_begin + p.per_split) : r_begin;
   const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh + (int64_t)key * p.kt;
-  u16x8 kf[L::KS], vf[L::KS];
+  u16x8 kf[L::KS], vf[kVInLds ? 1 : L::KS];
   load_row<DP>(kf, key < len ? kbase : nullptr, hh, p.D);
-  load_row<DP>(vf, key < len ? kbase + p.ks : nullptr, hh, p.D);
+  if constexpr (kVInLds) {  // each lane's half of its key's row, in the place that it reads again
+#pragma unroll
+    for (int k = 0; k < L::KS; ++k) {
+      const int col = 16 * k + 8 * hh;
+      *reinterpret_cast<u16x8*>(vs + L::off(wave * 32 + r, 2 * k + hh)) =
+          key < len && col < p.D ? *reinterpret_cast<const u16x8*>(kbase + p.ks + col) : zero8();
+    }
+  } else {
+    load_row<DP>(vf, key < len ? kbase + p.ks : nullptr, hh, p.D);
+  }
   f32x16 dk[L::NB], dv[L::NB];
 #pragma unroll
   for (int nb = 0; nb < L::NB; ++nb) dk[nb] = dv[nb] = zero16();
-  Stage<DP, RT> stage;
-  float sv = 0.f;
-  auto load = [&](int r0) {
-    stage.load(
-        [&](int which, int i) -> const u16* {
-          if (r0 + i >= r_end) return nullptr;
-          return which ? p.dout + p.dense_at(r0 + i, w.b, w.n) : p.q + p.row_at(r0 + i, w.b, w.n, p.qb, p.qt, p.qh);
-        },
-        p.D);
-    if (threadIdx.x < 2 * RT) {  // rows outside: P = 2^(0 - inf) = 0
-      const int i = threadIdx.x % RT;
-      const bool is_lse = threadIdx.x < RT;
-      sv = is_lse ? INFINITY : 0.f;
-      if (r0 + i < r_end) sv = (is_lse ? p.lse : p.delta)[(int64_t)w.bn * p.M + r0 + i];
-    }
+  const bool second = Copy::second(wave);
+  const int64_t H = (int64_t)p.N * p.G;
+  const u16* base = second ? p.dout + w.b * (p.Tq * H * p.D) + (int64_t)w.n * p.G * p.D
+                           : p.q + w.b * p.qb + (int64_t)w.n * p.G * p.qh;
+  const int64_t st = second ? H * p.D : p.qt, sh = second ? p.D : p.qh;
+  Copy copy;
+  // where a tile begins at a whole token, its rows lie alike in every tile
+  const bool alike = RT % p.G == 0;
+  auto offset = [&](int row) {
+    unsigned g;
+    const unsigned t = p.by_G.divmod((unsigned)row, g);
+    return (unsigned)(((int)t * (int)st + (int)g * (int)sh) * 2);
   };
-  auto store = [&](int buf) {
-    stage.store(smem[buf][0], smem[buf][1]);
-    if (threadIdx.x < 2 * RT) sstat[buf][threadIdx.x / RT][threadIdx.x % RT] = sv;
+  copy.init(wave, lane, p.D, offset);
+  const int mine = wave * kEach + lane;  // of the 2 RT statistics
+  auto issue = [&](Rows& t, int r0) {
+    const int at = r0 < r_end ? r0 : 0;
+    unsigned g;
+    const unsigned tok = p.by_G.divmod((unsigned)at, g);
+    if (!alike) copy.place(lane, p.D, [&](int row) { return offset(row + (int)g); });
+    copy.go(base + tok * st, t.x[second], r_end - r0);
+    const int i = mine % RT;
+    to_lds<4>((wave * kEach >= RT ? p.delta : p.lse) + (int64_t)w.bn * p.M + at, t.stat[wave],
+              lane < kEach && r0 + i < r_end ? (unsigned)(i * 4) : kOutside);
   };
-  if (r_begin < r_end) {
-    load(r_begin);
-    store(0);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int r0 = r_begin; r0 < r_end; r0 += RT, buf ^= 1) {
-    const bool more = r0 + RT < r_end;
-    if (more) load(r0 + RT);
-    const unsigned char *Qs = smem[buf][0], *Ds = smem[buf][1];
-    if (some) {
+  auto step = [&](const Rows& t, int r0) {
+    if (!some) return;
+    const unsigned char *Qs = t.x[0], *Ds = t.x[1];
+#pragma unroll 1
+    for (int qs = 0; qs < RT / 32; ++qs) {
+      f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int qs = 0; qs < RT / 32; ++qs) {
-        f32x16 s = zero16(), dp = zero16();
+      for (int k = 0; k < L::KS; ++k) {
+        s = mfma<E>(L::row8(Qs, qs * 32 + r, 2 * k + hh), kf[k], s);
+        dp = mfma<E>(L::row8(Ds, qs * 32 + r, 2 * k + hh), kVInLds ? L::row8(vs, wave * 32 + r, 2 * k + hh) : vf[kVInLds ? 0 : k], dp);
+      }
 #pragma unroll
-        for (int st = 0; st < L::KS; ++st) {
-          s = mfma<E>(L::row8(Qs, qs * 32 + r, 2 * st + hh), kf[st], s);
-          dp = mfma<E>(L::row8(Ds, qs * 32 + r, 2 * st + hh), vf[st], dp);
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const int qi = qs * 32 + 8 * g4 + 4 * hh;
+        const float4 l4 = *reinterpret_cast<const float4*>(&t.stat[qi / kEach][qi % kEach]);
+        const float4 d4 = *reinterpret_cast<const float4*>(&t.stat[(RT + qi) / kEach][qi % kEach]);
+        const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * g4 + j;
+          const float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -ls[j]));
+          s[i] = pv;
+          dp[i] = pv * (dp[i] - dl[j]);
         }
+      }
+      if (r0 + qs * 32 + 32 > r_end) {  // rows outside
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-          const int qi = qs * 32 + 8 * g4 + 4 * hh;
-          const float4 l4 = *reinterpret_cast<const float4*>(&sstat[buf][0][qi]);
-          const float4 d4 = *reinterpret_cast<const float4*>(&sstat[buf][1][qi]);
-          const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+        for (int i = 0; i < 16; ++i)
+          if (r0 + qs * 32 + acc_row(i, hh) >= r_end) s[i] = dp[i] = 0.f;
+      }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = 4 * g4 + j;
-            const float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -ls[j]));
-            s[i] = pv;
-            dp[i] = pv * (dp[i] - dl[j]);
-          }
-        }
+      for (int ks = 0; ks < 2; ++ks) {
+        const u16x8 pb = to_operand<E>(s, ks), db = to_operand<E>(dp, ks);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const u16x8 pb = to_operand<E>(s, ks), db = to_operand<E>(dp, ks);
-#pragma unroll
-          for (int nb = 0; nb < L::NB; ++nb) {
-            dv[nb] = mfma<E>(L::tr8(Ds, qs * 32 + 16 * ks, nb * 32, lane), pb, dv[nb]);
-            dk[nb] = mfma<E>(L::tr8(Qs, qs * 32 + 16 * ks, nb * 32, lane), db, dk[nb]);
-          }
+        for (int nb = 0; nb < L::NB; ++nb) {
+          dv[nb] = mfma<E>(L::tr8(Ds, qs * 32 + 16 * ks, nb * 32, lane), pb, dv[nb]);
+          dk[nb] = mfma<E>(L::tr8(Qs, qs * 32 + 16 * ks, nb * 32, lane), db, dk[nb]);
         }
       }
     }
-    if (more) store(buf ^ 1);
-    __syncthreads();
+  };
+  if (r_begin < r_end) {
+    if constexpr (L::BUFS == 3) pipeline<Copy::kPer + 1, RT>(tile0, tile1, tile2, r_begin, r_end, issue, step);
+    else pipeline<Copy::kPer + 1, RT>(tile0, tile1, r_begin, r_end, issue, step);
   }
   if (key >= p.Tk) return;
   // a lane whose key lies behind the last state has been computing with zeros for its key: its columns are not used
@@ -690,8 +836,6 @@ __global__ void __launch_bounds__(kThreads) cross_sum_kernel(const float* __rest
 }
 
 // ------------------------------------------------------------------------------ host side
-
-constexpr int kWanted = 512;  // workgroups that fill the chip: two on each of 256 CUs
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -777,8 +921,11 @@ std::vector<at::Tensor> cross_fwd(const at::Tensor& q, const at::Tensor& kv, con
       hipLaunchKernelGGL((cross_fwd_kernel<E, dp>), dim3(grid), dim3(kThreads), 0, stream(), p);
     LAUNCH_CHECK();
     if (p.splits > 1) {
-      const int64_t items = (int64_t)p.B * p.N * p.M * (p.D / 4);
-      hipLaunchKernelGGL((cross_join_kernel<E>), dim3((unsigned)up(items, kThreads)), dim3(kThreads), 0, stream(), p, items);
+      const int64_t rows = (int64_t)p.B * p.N * p.M;
+      if (p.splits > 16)
+        hipLaunchKernelGGL((cross_join_kernel<E, 256>), dim3((unsigned)rows), dim3(256), 0, stream(), p);
+      else
+        hipLaunchKernelGGL((cross_join_kernel<E, 64>), dim3((unsigned)rows), dim3(64), 0, stream(), p);
       LAUNCH_CHECK();
     }
   });
@@ -831,10 +978,13 @@ std::vector<at::Tensor> cross_bwd(const at::Tensor& dout, const at::Tensor& q, c
   return {dq, dkv};
 }
 
-// Rows of whole 16-byte chunks at 16-byte addresses, or a copy that has them.
+// Rows of whole 16-byte chunks at 16-byte addresses whose tiles stay within the copies' 31-bit offsets (tokens of
+// one tile, and the heads of a group), or a dense copy that has them.
 at::Tensor chunked(const at::Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) ok &= t.size(i) == 1 || t.stride(i) % 8 == 0;
+  const int64_t heads = t.dim() - 2;
+  ok &= 2 * (kRows * t.stride(1) + t.size(heads) * t.stride(heads) + t.size(-1)) < (1ll << 30);
   if (ok) return t;
   auto c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);

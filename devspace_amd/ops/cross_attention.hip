@@ -63,18 +63,36 @@ struct Tile {
     if constexpr (RB == 128) return row * 128 + ((chunk ^ ((row >> 1) & 7) ^ ((row & 2) << 1)) << 4);
     else return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
   }
-  __device__ static __forceinline__ u16x8 row8(const unsigned char* tile, int row, int chunk) {
-    return *reinterpret_cast<const u16x8*>(tile + off(row, chunk));
+};
+
+// A lane's places in a tile, the same in every tile and (32 and 16 rows being whole periods of the swizzle) in
+// every block of rows: kept in registers, all else is a constant of the instruction.
+template <int DP>
+struct Places {
+  typedef Tile<DP> L;
+  int row[L::KS];    // chunk 2 s + hh of row r (r = lane & 31, hh = lane >> 5)
+  int tr[L::NB][2];  // the transposed operand's four rows from 4 hh on and from 8 + 4 hh on, 32 columns at nb 32
+  __device__ __forceinline__ explicit Places(int lane) {
+    const int r = lane & 31, hh = lane >> 5, g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int s = 0; s < L::KS; ++s) row[s] = L::off(r, 2 * s + hh);
+#pragma unroll
+    for (int nb = 0; nb < L::NB; ++nb) {
+      const int col = nb * 32 + 16 * (g & 1) + 4 * (i & 3);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) tr[nb][k] = L::off(8 * k + 4 * hh + (i >> 2), col >> 3) + ((col & 7) << 1);
+    }
   }
-  // Operand of the transposed tile: lane (r = lane & 31, hh = lane >> 5) gets column col0 + r of rows
-  // r0 + 4 hh + {0..3} and r0 + 8 + 4 hh + {0..3}: the order of an accumulator's rows.
-  __device__ static __forceinline__ u16x8 tr8(const unsigned char* tile, int r0, int col0, int lane) {
-    const int g = lane >> 4, i = lane & 15, hh = lane >> 5;
-    const int row = r0 + 4 * hh + (i >> 2);
-    const int col = col0 + 16 * (g & 1) + 4 * (i & 3);
-    lds_u8* base = (lds_u8*)tile;
-    s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + off(row, col >> 3) + ((col & 7) << 1)));
-    s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + off(row + 8, col >> 3) + ((col & 7) << 1)));
+  // columns 16 s + 8 hh .. of row r0 + r; r0 a multiple of 32
+  __device__ __forceinline__ u16x8 row8(const unsigned char* tile, int r0, int s) const {
+    return *reinterpret_cast<const u16x8*>(tile + row[s] + r0 * L::RB);
+  }
+  // Operand of the transposed tile: column nb 32 + r of rows r0 + 4 hh + {0..3} and r0 + 8 + 4 hh + {0..3}, the
+  // order of an accumulator's rows; r0 a multiple of 16.
+  __device__ __forceinline__ u16x8 tr8(const unsigned char* tile, int r0, int nb) const {
+    lds_u8* base = (lds_u8*)tile + r0 * L::RB;
+    s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + tr[nb][0]));
+    s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + tr[nb][1]));
     return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
@@ -230,30 +248,53 @@ __device__ __forceinline__ void load_row(u16x8* f, const u16* row, int hh, int D
   }
 }
 
-// One tile of scores in the log2 domain: the online softmax of this lane's row. On return s holds P.
-template <int KB>
-__device__ __forceinline__ float soften(f32x16* s, float& m, float& l, float scale_log2) {
+// the larger, or the sum, of this lane's value and that of the other half's lane of the same row
+__device__ __forceinline__ void other_half(float x, float& a, float& b) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  a = __uint_as_float(both[0]);
+  b = __uint_as_float(both[1]);
+}
+__device__ __forceinline__ float half_max(float x) {
+  float a, b;
+  other_half(x, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float x) {
+  float a, b;
+  other_half(x, a, b);
+  return a + b;
+}
+
+// One tile of scores in the log2 domain: the online softmax of this lane's row. On return s holds P against the
+// reference m, which follows the running maximum only when that has left it by more than 2^8: P and the sums stay
+// within 2^8 times the number of keys, nothing is lost in their floating types, and O (64 registers with wide
+// heads) is rarely rescaled. In front of the exponentials, `rescale` gets the factor where any row moves.
+template <int KB, typename F>
+__device__ __forceinline__ void soften(f32x16* s, float& m, float& l, float scale_log2, F&& rescale) {
   float mt = -INFINITY;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
-  mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-  const float mn = fmaxf(m, mt * scale_log2);
-  const float base = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: all of P is 0
-  const float alpha = exp2_fast(m - base);
-  float ls = 0.f;
+  mt = half_max(mt) * scale_log2;
+  if (__any(mt > m + 8.f)) {
+    const float mn = fmaxf(m, mt);
+    const float alpha = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
+    l *= alpha;
+    m = mn;
+    rescale(alpha);
+  }
+  const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: all of P is 0
+  float ls[2] = {0.f, 0.f};
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float e = exp2_fast(__builtin_fmaf(s[kb][i], scale_log2, -base));
       s[kb][i] = e;
-      ls += e;
+      ls[i & 1] += e;
     }
-  l = l * alpha + ls;
-  m = mn;
-  return alpha;
+  l += ls[0] + ls[1];
 }
 
 // Four columns of a row of O^T or dQ^T accumulators at a time: column nb 32 + 8 g4 + 4 hh
@@ -350,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
   const Place w(p);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, hh = lane >> 5;
+  const Places<DP> lds(lane);
   const int m0 = w.block * kRows + wave * 32, row = m0 + r;
   const bool some = m0 < p.M;  // the wave has rows at all
   const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
@@ -365,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
 #pragma unroll
     for (int st = 0; st < L::KS; ++st)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) s[kb] = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s[kb]);
+      for (int kb = 0; kb < 2; ++kb) s[kb] = mfma<E>(lds.row8(Ks, kb * 32, st), qf[st], s[kb]);
     if (k0 + kKeys > k_end) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -373,28 +415,27 @@ __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
         for (int i = 0; i < 16; ++i)
           if (k0 + kb * 32 + acc_row(i, hh) >= k_end) s[kb][i] = -INFINITY;
     }
-    const float alpha = soften<2>(s, m, l, p.scale_log2);
-    if (__any(alpha != 1.f)) {  // some row of the wave has a new maximum
+    soften<2>(s, m, l, p.scale_log2, [&](float alpha) {
 #pragma unroll
       for (int nb = 0; nb < L::NB; ++nb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
-    }
+    });
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       const u16x8 pb = to_operand<E>(s[ks >> 1], ks & 1);
 #pragma unroll
-      for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(L::tr8(Vs, 16 * ks, nb * 32, lane), pb, o[nb]);
+      for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(lds.tr8(Vs, 16 * ks, nb), pb, o[nb]);
     }
   };
   key_loop<DP>(tile0, tile1, tile2, p, w, wave, lane, k_begin, k_end, step);
   if (row >= p.M) return;
-  l += __shfl_xor(l, 32, 64);
+  l = half_sum(l);
   const int64_t stat = (int64_t)w.bn * p.M + row;
   if (p.splits == 1) {
     const float inv = k_begin < k_end ? 1.f / l : 0.f;  // no state at all: 0
-    u16* at = p.out + p.dense_at(row, w.b, w.n);
-    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4<E>(at + col, o[nb], i, inv); });
+    u16* to = p.out + p.dense_at(row, w.b, w.n);
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4<E>(to + col, o[nb], i, inv); });
     if (p.lse && hh == 0) p.lse[stat] = m + __log2f(l);
   } else if (k_begin < k_end) {
     const int64_t at = ((int64_t)w.split * p.B * p.N + w.bn) * p.M + row;
@@ -420,6 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   const Place w(p);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 31, hh = lane >> 5;
+  const Places<DP> lds(lane);
   const int m0 = w.block * 32, row = m0 + r;
   const int rows = min(32, p.M - m0);
   const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
@@ -463,11 +505,12 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
       for (int i = 0; i < 16; ++i)
         if (k0 + acc_row(i, hh) >= k_end) s[i] = -INFINITY;
     }
-    const float alpha = soften<1>(&s, m, l, p.scale_log2);
+    soften<1>(&s, m, l, p.scale_log2, [&](float alpha) {
 #pragma unroll
-    for (int nb = 0; nb < L::NB; ++nb)
+      for (int nb = 0; nb < L::NB; ++nb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
+        for (int i = 0; i < 16; ++i) o[nb][i] *= alpha;
+    });
     // the tile belongs to this wave alone, and a wave's LDS operations stay in order
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -476,14 +519,14 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
     for (int ks = 0; ks < 2; ++ks) {
       const u16x8 pb = to_operand<E>(s, ks);
 #pragma unroll
-      for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(L::tr8(Vs, 16 * ks, nb * 32, lane), pb, o[nb]);
+      for (int nb = 0; nb < L::NB; ++nb) o[nb] = mfma<E>(lds.tr8(Vs, 16 * ks, nb), pb, o[nb]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
   // join the four waves: their maxima and sums, then their rows on the common maximum
-  l += __shfl_xor(l, 32, 64);
+  l = half_sum(l);
   if (hh == 0) {
     sml[wave][0][r] = m;
     sml[wave][1][r] = l;
@@ -600,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   const Place w(p);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, hh = lane >> 5;
+  const Places<DP> lds(lane);
   const int m0 = w.block * kRows + wave * 32, row = m0 + r;
   const bool some = m0 < p.M, mine = row < p.M;
   const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
@@ -612,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   for (int s = 0; s < L::KS; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta += E::get(df[s][j]) * E::get(qf[s][j]);
-  delta += __shfl_xor(delta, 32, 64);
+  delta = half_sum(delta);
   const float lse = mine ? p.lse[stat] : INFINITY;  // rows outside: P = 2^(0 - inf) = 0
   load_row<DP>(qf, mine ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
   f32x16 dq[L::NB];
@@ -624,8 +668,8 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
     dp = zero16();
 #pragma unroll
     for (int st = 0; st < L::KS; ++st) {
-      s = mfma<E>(L::row8(Ks, kb * 32 + r, 2 * st + hh), qf[st], s);
-      dp = mfma<E>(L::row8(Vs, kb * 32 + r, 2 * st + hh), df[st], dp);
+      s = mfma<E>(lds.row8(Ks, kb * 32, st), qf[st], s);
+      dp = mfma<E>(lds.row8(Vs, kb * 32, st), df[st], dp);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse));
@@ -642,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
     for (int ks = 0; ks < 2; ++ks) {
       const u16x8 db = to_operand<E>(dp, ks);
 #pragma unroll
-      for (int nb = 0; nb < L::NB; ++nb) dq[nb] = mfma<E>(L::tr8(Ks, kb * 32 + 16 * ks, nb * 32, lane), db, dq[nb]);
+      for (int nb = 0; nb < L::NB; ++nb) dq[nb] = mfma<E>(lds.tr8(Ks, kb * 32 + 16 * ks, nb), db, dq[nb]);
     }
   };
   if (p.splits == 1 && k_end <= kKeys) {
@@ -658,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += s[i] * dp[i];
       }
-      delta = sum + __shfl_xor(sum, 32, 64);
+      delta = half_sum(sum);
 #pragma unroll 1
       for (int kb = 0; kb < 2; ++kb) {
         scores(Ks, Vs, k0, kb, s, dp);
@@ -703,6 +747,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   const Place w(p);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, hh = lane >> 5;
+  const Places<DP> lds(lane);
   const int kw = w.block * kRows + wave * 32, key = kw + r;
   const int len = p.length(w.b);
   const bool some = kw < len;
@@ -741,13 +786,13 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   copy.init(wave, lane, p.D, offset);
   const int mine = wave * kEach + lane;  // of the 2 RT statistics
   auto issue = [&](Rows& t, int r0) {
-    const int at = r0 < r_end ? r0 : 0;
+    const int begin = r0 < r_end ? r0 : 0;
     unsigned g;
-    const unsigned tok = p.by_G.divmod((unsigned)at, g);
+    const unsigned tok = p.by_G.divmod((unsigned)begin, g);
     if (!alike) copy.place(lane, p.D, [&](int row) { return offset(row + (int)g); });
     copy.go(base + tok * st, t.x[second], r_end - r0);
     const int i = mine % RT;
-    to_lds<4>((wave * kEach >= RT ? p.delta : p.lse) + (int64_t)w.bn * p.M + at, t.stat[wave],
+    to_lds<4>((wave * kEach >= RT ? p.delta : p.lse) + (int64_t)w.bn * p.M + begin, t.stat[wave],
               lane < kEach && r0 + i < r_end ? (unsigned)(i * 4) : kOutside);
   };
   auto step = [&](const Rows& t, int r0) {
@@ -758,8 +803,8 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int k = 0; k < L::KS; ++k) {
-        s = mfma<E>(L::row8(Qs, qs * 32 + r, 2 * k + hh), kf[k], s);
-        dp = mfma<E>(L::row8(Ds, qs * 32 + r, 2 * k + hh), kVInLds ? L::row8(vs, wave * 32 + r, 2 * k + hh) : vf[kVInLds ? 0 : k], dp);
+        s = mfma<E>(lds.row8(Qs, qs * 32, k), kf[k], s);
+        dp = mfma<E>(lds.row8(Ds, qs * 32, k), kVInLds ? lds.row8(vs, wave * 32, k) : vf[kVInLds ? 0 : k], dp);
       }
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4) {
@@ -785,8 +830,8 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
         const u16x8 pb = to_operand<E>(s, ks), db = to_operand<E>(dp, ks);
 #pragma unroll
         for (int nb = 0; nb < L::NB; ++nb) {
-          dv[nb] = mfma<E>(L::tr8(Ds, qs * 32 + 16 * ks, nb * 32, lane), pb, dv[nb]);
-          dk[nb] = mfma<E>(L::tr8(Qs, qs * 32 + 16 * ks, nb * 32, lane), db, dk[nb]);
+          dv[nb] = mfma<E>(lds.tr8(Ds, qs * 32 + 16 * ks, nb), pb, dv[nb]);
+          dk[nb] = mfma<E>(lds.tr8(Qs, qs * 32 + 16 * ks, nb), db, dk[nb]);
         }
       }
     }

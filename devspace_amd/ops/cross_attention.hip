@@ -175,23 +175,40 @@ struct Place {
   }
 };
 
-// One wave's share of copying tiles of ROWS rows of two tensors (waves 0 and 1 the first, 2 and 3 the second)
-// straight into LDS: buffer loads that write there without passing registers, 64 lanes x 16 bytes, a few whole
-// rows each. The swizzle is applied to the source: lane l fills the l-th 16 bytes and fetches the chunk that
-// belongs there. Rows and columns outside get an offset beyond the buffer, which reads as 0.
+// Buffer loads know how many bytes there are from their base on, and read 0 behind them: tiles that reach past
+// the last row, and columns past D (whose lanes get the offset kOutside), need no branches.
 constexpr unsigned kOutside = 0x80000000u;
 
-// BYTES (4 or 16) per lane from `base` plus this lane's offset to `lds` plus BYTES times the lane
+// bytes from a tile's first row to the end of its last valid one; none for valid <= 0
+__device__ __forceinline__ unsigned bytes_of(int valid, int64_t stride, int D) {
+  return valid <= 0 ? 0u : (unsigned)min(((int64_t)(valid - 1) * stride + D) * 2, (int64_t)kOutside - 1);
+}
+
+// BYTES (4 or 16) per lane from `base` plus this lane's offset to `lds` plus BYTES times the lane, without passing
+// registers
 template <int BYTES>
-__device__ __forceinline__ void to_lds(const void* base, void* lds, unsigned offset) {
-#ifdef __HIP_DEVICE_COMPILE__  // the buffer's type is the device's
-  __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, kOutside - 1, 0x00020000);
+__device__ __forceinline__ void to_lds(const void* base, unsigned bytes, void* lds, unsigned offset) {
   static_assert(BYTES == 16 || BYTES == 4, "sizes used here");
+#ifdef __HIP_DEVICE_COMPILE__  // the buffer's type is the device's
+  __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
   if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(lds_u8*)lds, 16, offset, 0, 0, 0);
   else __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(lds_u8*)lds, 4, offset, 0, 0, 0);
 #endif
 }
 
+// N chunks of 16 bytes at this lane's offsets
+template <int N>
+__device__ __forceinline__ void to_registers(u16x8 (&to)[N], const void* base, unsigned bytes, const unsigned (&offset)[N]) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+#pragma unroll
+  for (int u = 0; u < N; ++u) to[u] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(src, offset[u], 0, 0));
+#endif
+}
+
+// One wave's share of copying tiles of ROWS rows of two tensors (waves 0 and 1 the first, 2 and 3 the second)
+// into LDS: 64 lanes x 16 bytes, a few whole rows each. The swizzle is applied to the source: lane l fills the
+// l-th 16 bytes and fetches the chunk that belongs there.
 template <int DP, int ROWS>
 struct Dma {
   typedef Tile<DP> L;
@@ -199,32 +216,27 @@ struct Dma {
   static constexpr int kRowsEach = 1024 / L::RB;
   static constexpr int kSlots = L::RB / 16;
   unsigned at[kPer];  // byte offset of this lane's chunk from the tile's first row
-  int first;          // this lane's row in the wave's first load
   int piece;          // where the wave's part of a tensor's tile begins, bytes
 
   __device__ static __forceinline__ bool second(int wave) { return wave >= 2; }
-
-  // offset(row): byte offset of a row of the tile
-  template <typename F>
-  __device__ __forceinline__ void init(int wave, int lane, int D, F&& offset) {
-    first = (wave & 1) * (ROWS / 2) + lane / kSlots;
-    piece = (wave & 1) * (ROWS / 2) * L::RB;
-    place(lane, D, offset);
+  __device__ static __forceinline__ int row(int wave, int lane, int u) {
+    return (wave & 1) * (ROWS / 2) + u * kRowsEach + lane / kSlots;
   }
+  // offset(row): byte offset of a row of the tile, or kOutside
   template <typename F>
-  __device__ __forceinline__ void place(int lane, int D, F&& offset) {
+  __device__ __forceinline__ void place(int wave, int lane, int D, F&& offset) {
+    piece = (wave & 1) * (ROWS / 2) * L::RB;
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
-      const int row = first + u * kRowsEach;
-      const int chunk = (L::off(row, lane % kSlots) - row * L::RB) >> 4;
-      at[u] = chunk * 8 < D ? offset(row) + chunk * 16 : kOutside;
+      const int i = row(wave, lane, u);
+      const int chunk = (L::off(i, lane % kSlots) - i * L::RB) >> 4;
+      const unsigned o = offset(i);
+      at[u] = chunk * 8 < D && o < kOutside ? o + chunk * 16 : kOutside;
     }
   }
-  // rows [0, valid) of the tile that begins at `base`; valid <= 0 fills the tile with zeros
-  __device__ __forceinline__ void go(const u16* base, unsigned char* tile, int valid) const {
+  __device__ __forceinline__ void go(const u16* base, unsigned bytes, unsigned char* tile) const {
 #pragma unroll
-    for (int u = 0; u < kPer; ++u)
-      to_lds<16>(base, tile + piece + u * 1024, first + u * kRowsEach < valid ? at[u] : kOutside);
+    for (int u = 0; u < kPer; ++u) to_lds<16>(base, bytes, tile + piece + u * 1024, at[u]);
   }
 };
 
@@ -373,10 +385,10 @@ __device__ __forceinline__ void key_loop(KeyTile<DP>& tile0, KeyTile<DP>& tile1,
   typedef KeyTile<DP> Pair;
   if (begin >= end) return;
   Copy copy;
-  copy.init(wave, lane, p.D, [&](int row) { return (unsigned)(row * (int)p.kt * 2); });
+  copy.place(wave, lane, p.D, [&](int row) { return (unsigned)(row * (int)p.kt * 2); });
   const bool second = Copy::second(wave);
   const u16* base = p.kv + w.b * p.kb + w.n * p.kh + (second ? p.ks : 0);
-  auto issue = [&](Pair& t, int k0) { copy.go(base + (k0 < end ? k0 : 0) * p.kt, t[second], end - k0); };
+  auto issue = [&](Pair& t, int k0) { copy.go(base + (k0 < end ? k0 : 0) * p.kt, bytes_of(end - k0, p.kt, p.D), t[second]); };
   auto use = [&](const Pair& t, int k0) { step(t[0], t[1], k0); };
   if constexpr (L::BUFS == 3) pipeline<Copy::kPer, kKeys>(tile0, tile1, tile2, begin, end, issue, use);
   else pipeline<Copy::kPer, kKeys>(tile0, tile1, begin, end, issue, use);
@@ -466,40 +478,40 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   const int rows = min(32, p.M - m0);
   const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
   const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh;
-  u16x8 qf[L::KS], kf[L::KS], vr[kPer];
+  u16x8 qf[L::KS];
   load_row<DP>(qf, row < p.M ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
   f32x16 o[L::NB];
 #pragma unroll
   for (int nb = 0; nb < L::NB; ++nb) o[nb] = zero16();
   float m = -INFINITY, l = 0.f;
   unsigned char* Vs = sm.v[wave];
-  auto load_k = [&](int k0) {
-    load_row<DP>(kf, k0 + r < k_end ? kbase + (int64_t)(k0 + r) * p.kt : nullptr, hh, p.D);
-  };
-  auto load_v = [&](int k0) {
+  unsigned at_k[L::KS], at_v[kPer];
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const int c = lane + 64 * u, key = k0 + c / L::CH, ch = c % L::CH;
-      vr[u] = key < k_end && ch * 8 < p.D ? *reinterpret_cast<const u16x8*>(kbase + (int64_t)key * p.kt + p.ks + ch * 8) : zero8();
-    }
-  };
-  int k0 = k_begin + wave * kTile;
-  if (k0 < k_end) {
-    load_k(k0);
-    load_v(k0);
+  for (int st = 0; st < L::KS; ++st) at_k[st] = 16 * st + 8 * hh < p.D ? (unsigned)(r * (int)p.kt + 16 * st + 8 * hh) * 2 : kOutside;
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int c = lane + 64 * u, ch = c % L::CH;
+    at_v[u] = ch * 8 < p.D ? (unsigned)(c / L::CH * (int)p.kt + ch * 8) * 2 : kOutside;
   }
-  for (; k0 < k_end; k0 += 4 * kTile) {
-    const int next = k0 + 4 * kTile;
+  struct Keys {  // one tile on its way: keys as operands, values by rows
+    u16x8 k[L::KS], v[kPer];
+  };
+  auto load = [&](Keys& t, int k0) {
+    const u16* base = kbase + (k0 < k_end ? k0 : 0) * p.kt;
+    const unsigned bytes = bytes_of(k_end - k0, p.kt, p.D);
+    to_registers(t.k, base, bytes, at_k);
+    to_registers(t.v, base + p.ks, bytes, at_v);
+  };
+  auto step = [&](Keys& t, int k0, int ahead) {
     f32x16 s = zero16();
 #pragma unroll
-    for (int st = 0; st < L::KS; ++st) s = mfma<E>(kf[st], qf[st], s);
-    if (next < k_end) load_k(next);
+    for (int st = 0; st < L::KS; ++st) s = mfma<E>(t.k[st], qf[st], s);
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int c = lane + 64 * u;
-      *reinterpret_cast<u16x8*>(Vs + L::off(c / L::CH, c % L::CH)) = vr[u];
+      *reinterpret_cast<u16x8*>(Vs + L::off(c / L::CH, c % L::CH)) = t.v[u];
     }
-    if (next < k_end) load_v(next);
+    load(t, k0 + ahead);
     if (k0 + kTile > k_end) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -524,6 +536,22 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  // the loads of one more tile, or of two where the registers hold them, are under way
+  constexpr int kStride = 4 * kTile;
+  int k0 = __builtin_amdgcn_readfirstlane(k_begin + wave * kTile);
+  Keys t0, t1;
+  load(t0, k0);
+  if constexpr (L::BUFS == 3) {
+    load(t1, k0 + kStride);
+    while (k0 < k_end) {
+      step(t0, k0, 2 * kStride);
+      if ((k0 += kStride) >= k_end) break;
+      step(t1, k0, 2 * kStride);
+      k0 += kStride;
+    }
+  } else {
+    for (; k0 < k_end; k0 += kStride) step(t0, k0, kStride);
   }
   // join the four waves: their maxima and sums, then their rows on the common maximum
   l = half_sum(l);
@@ -776,24 +804,26 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
                            : p.q + w.b * p.qb + (int64_t)w.n * p.G * p.qh;
   const int64_t st = second ? H * p.D : p.qt, sh = second ? p.D : p.qh;
   Copy copy;
-  // where a tile begins at a whole token, its rows lie alike in every tile
+  // Offsets of a tile's rows from its first token. Where tiles begin at whole tokens they are the same in every
+  // tile but for the last, whose rows outside are struck out.
   const bool alike = RT % p.G == 0;
-  auto offset = [&](int row) {
-    unsigned g;
-    const unsigned t = p.by_G.divmod((unsigned)row, g);
-    return (unsigned)(((int)t * (int)st + (int)g * (int)sh) * 2);
+  auto place = [&](int skipped, int valid) {
+    copy.place(wave, lane, p.D, [&](int i) {
+      unsigned g;
+      const unsigned t = p.by_G.divmod((unsigned)(i + skipped), g);
+      return i < valid ? (unsigned)(((int)t * (int)st + (int)g * (int)sh) * 2) : kOutside;
+    });
   };
-  copy.init(wave, lane, p.D, offset);
+  place(0, RT);
   const int mine = wave * kEach + lane;  // of the 2 RT statistics
   auto issue = [&](Rows& t, int r0) {
-    const int begin = r0 < r_end ? r0 : 0;
-    unsigned g;
-    const unsigned tok = p.by_G.divmod((unsigned)begin, g);
-    if (!alike) copy.place(lane, p.D, [&](int row) { return offset(row + (int)g); });
-    copy.go(base + tok * st, t.x[second], r_end - r0);
-    const int i = mine % RT;
-    to_lds<4>((wave * kEach >= RT ? p.delta : p.lse) + (int64_t)w.bn * p.M + begin, t.stat[wave],
-              lane < kEach && r0 + i < r_end ? (unsigned)(i * 4) : kOutside);
+    const int begin = r0 < r_end ? r0 : 0, valid = r_end - r0;
+    unsigned skipped;
+    const unsigned token = p.by_G.divmod((unsigned)begin, skipped);
+    if (!alike || (valid > 0 && valid < RT)) place((int)skipped, valid);
+    copy.go(base + token * st, valid > 0 ? kOutside - 1 : 0u, t.x[second]);
+    to_lds<4>((wave * kEach >= RT ? p.delta : p.lse) + (int64_t)w.bn * p.M + begin, valid > 0 ? 4u * min(valid, RT) : 0u,
+              t.stat[wave], lane < kEach ? (unsigned)(mine % RT * 4) : kOutside);
   };
   auto step = [&](const Rows& t, int r0) {
     if (!some) return;
@@ -1028,6 +1058,7 @@ std::vector<at::Tensor> cross_bwd(const at::Tensor& dout, const at::Tensor& q, c
 at::Tensor chunked(const at::Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) ok &= t.size(i) == 1 || t.stride(i) % 8 == 0;
+  ok &= t.size(1) == 1 || t.stride(1) >= t.size(-1);  // a tile's rows end in their order
   const int64_t heads = t.dim() - 2;
   ok &= 2 * (kRows * t.stride(1) + t.size(heads) * t.stride(heads) + t.size(-1)) < (1ll << 30);
   if (ok) return t;

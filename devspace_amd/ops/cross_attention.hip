@@ -892,32 +892,45 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   }
 }
 
-// out[i] = sum over parts of part[s][i], in their order; numel is a multiple of 8
+struct PartSum {  // out[i] = sum over parts of part[s][i], in their order
+  const float* part;
+  u16* out;
+  int64_t numel;  // a multiple of 8
+  int parts;      // 0: nothing to add
+  int blocks;
+};
+
+// the split dQ's and the split dK's and dV's sums, one launch
 template <typename E>
-__global__ void __launch_bounds__(kThreads) cross_sum_kernel(const float* __restrict__ part, u16* __restrict__ out,
-                                                             int64_t numel, int parts) {
-  const int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8;
-  if (at >= numel) return;
+__global__ void __launch_bounds__(kThreads) cross_sum_kernel(PartSum first, PartSum second) {
+  const bool one = (int)blockIdx.x < first.blocks;
+  const PartSum& j = one ? first : second;
+  const int64_t at = ((int64_t)(blockIdx.x - (one ? 0 : first.blocks)) * kThreads + threadIdx.x) * 8;
+  if (at >= j.numel) return;
   float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < parts; ++s) {
-    const auto v = load_pack<float, 8>(part + s * numel + at);
+  for (int s = 0; s < j.parts; ++s) {
+    const auto v = load_pack<float, 8>(j.part + s * j.numel + at);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] += v.v[j];
+    for (int i = 0; i < 8; ++i) a[i] += v.v[i];
   }
   u16x8 o;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = E::put(a[j]);
-  *reinterpret_cast<u16x8*>(out + at) = o;
+  for (int i = 0; i < 8; ++i) o[i] = E::put(a[i]);
+  *reinterpret_cast<u16x8*>(j.out + at) = o;
 }
 
 // ------------------------------------------------------------------------------ host side
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Splits an axis of `len` into parts of whole tiles so that `have` workgroups become about kWanted.
-void split_axis(CrossParams& p, int64_t have, int len, int tile, int least) {
-  int splits = (int)std::max<int64_t>(1, std::min<int64_t>(kWanted / std::max<int64_t>(1, have), up(len, least)));
-  p.per_split = std::max(tile, up(up(len, splits), tile) * tile);
+// Splits an axis of `len` into parts of whole tiles, each of four at least, so that `have` workgroups become about
+// kWanted. A tile takes a workgroup about 1.2 us and joining the parts one more launch of about 5 us (1848 rows x 80
+// over 1499 keys: forward 9.7 us and 4.4 us of joining in six parts, about 30 us in one), so that an axis of fewer
+// than twelve tiles stays whole.
+void split_axis(CrossParams& p, int64_t have, int len, int tile) {
+  const int tiles = up(len, tile);
+  const int splits = tiles < 12 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(kWanted / std::max<int64_t>(1, have), tiles / 4));
+  p.per_split = std::max(1, up(tiles, splits)) * tile;
   p.splits = std::max(1, up(len, p.per_split));
 }
 
@@ -980,7 +993,7 @@ std::vector<at::Tensor> cross_fwd(const at::Tensor& q, const at::Tensor& kv, con
   p.lse = with_lse ? lse.data_ptr<float>() : nullptr;
   const bool few = p.M <= 32;
   p.blocks = up(p.M, few ? 32 : kRows);
-  split_axis(p, (int64_t)p.blocks * p.B * p.N, p.Tk, few ? 128 : kKeys, 256);
+  split_axis(p, (int64_t)p.blocks * p.B * p.N, p.Tk, few ? 128 : kKeys);
   if (p.splits > 1) {
     part = at::empty({p.splits, (int64_t)p.B * p.N * p.M * p.D}, f32);
     ml = at::empty({p.splits, (int64_t)p.B * p.N * p.M, 2}, f32);
@@ -1013,42 +1026,38 @@ std::vector<at::Tensor> cross_bwd(const at::Tensor& dout, const at::Tensor& q, c
   CrossParams p = cross_params(q, kv, lengths, scale);
   auto dq = at::empty(q.sizes(), q.options()), dkv = at::empty(kv.sizes(), kv.options());
   if (q.numel() == 0 || kv.numel() == 0) return {dq.zero_(), dkv.zero_()};
-  const auto f32 = q.options().dtype(at::kFloat);
-  auto delta = at::empty({p.B, p.N, p.M}, f32);
   p.o = (const u16*)out.data_ptr();
   p.dout = (const u16*)dout.data_ptr();
   p.out = (u16*)dq.data_ptr();
   p.dkv = (u16*)dkv.data_ptr();
   p.lse = lse.data_ptr<float>();
-  p.delta = delta.data_ptr<float>();
   by_type_and_width(p, q.scalar_type(), [&](auto e, auto dp) {
     typedef decltype(e) E;
     constexpr int RT = dp <= 64 ? 64 : 32;
-    auto sum = [&](const at::Tensor& part, at::Tensor& to) {
-      const int64_t n = to.numel();
-      hipLaunchKernelGGL((cross_sum_kernel<E>), dim3((unsigned)up(n, 8 * kThreads)), dim3(kThreads), 0, stream(),
-                         part.data_ptr<float>(), (u16*)to.data_ptr(), n, p.splits);
-      LAUNCH_CHECK();
-    };
-    at::Tensor part;
+    CrossParams pk = p;  // dK, dV
     p.blocks = up(p.M, kRows);
-    split_axis(p, (int64_t)p.blocks * p.B * p.N, p.Tk, kKeys, 256);
-    if (p.splits > 1) {
-      part = at::empty({p.splits, p.out_numel}, f32);
-      p.part = part.data_ptr<float>();
-    }
+    split_axis(p, (int64_t)p.blocks * p.B * p.N, p.Tk, kKeys);
+    pk.blocks = up(p.Tk, kRows);
+    split_axis(pk, (int64_t)pk.blocks * p.B * p.N, p.M, RT);
+    // one workspace: the rows' sums of dP, then the parts of split gradients
+    const int64_t rows = ((int64_t)p.B * p.N * p.M + 7) / 8 * 8;
+    const int64_t nq = p.splits > 1 ? p.splits * p.out_numel : 0, nkv = pk.splits > 1 ? pk.splits * p.dkv_numel : 0;
+    auto work = at::empty({rows + nq + nkv}, q.options().dtype(at::kFloat));
+    p.delta = pk.delta = work.data_ptr<float>();
+    p.part = p.delta + rows;
+    pk.part = p.part + nq;
     hipLaunchKernelGGL((cross_dq_kernel<E, dp>), dim3(grid_of(p)), dim3(kThreads), 0, stream(), p);
     LAUNCH_CHECK();
-    if (p.splits > 1) sum(part, dq);
-    p.blocks = up(p.Tk, kRows);
-    split_axis(p, (int64_t)p.blocks * p.B * p.N, p.M, RT, 128);
-    if (p.splits > 1) {
-      part = at::empty({p.splits, p.dkv_numel}, f32);
-      p.part = part.data_ptr<float>();
-    }
-    hipLaunchKernelGGL((cross_dkv_kernel<E, dp, RT>), dim3(grid_of(p)), dim3(kThreads), 0, stream(), p);
+    hipLaunchKernelGGL((cross_dkv_kernel<E, dp, RT>), dim3(grid_of(pk)), dim3(kThreads), 0, stream(), pk);
     LAUNCH_CHECK();
-    if (p.splits > 1) sum(part, dkv);
+    auto job = [](const CrossParams& c, u16* to, int64_t n) {
+      return PartSum{c.part, to, n, c.splits, c.splits > 1 ? up(n, 8 * kThreads) : 0};
+    };
+    const PartSum a = job(p, p.out, p.out_numel), b = job(pk, pk.dkv, pk.dkv_numel);
+    if (a.blocks + b.blocks > 0) {
+      hipLaunchKernelGGL((cross_sum_kernel<E>), dim3((unsigned)(a.blocks + b.blocks)), dim3(kThreads), 0, stream(), a, b);
+      LAUNCH_CHECK();
+    }
   });
   return {dq, dkv};
 }

@@ -1021,15 +1021,16 @@ std::vector<at::Tensor> cross_fwd(const at::Tensor& q, const at::Tensor& kv, con
 }
 
 std::vector<at::Tensor> cross_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& kv, const at::Tensor& out,
-                                  const at::Tensor& lse, const OptTensor& lengths, double scale) {
+                                  const at::Tensor& lse, const OptTensor& lengths, double scale, bool want_kv) {
   c10::DeviceGuard guard(q.device());
   CrossParams p = cross_params(q, kv, lengths, scale);
-  auto dq = at::empty(q.sizes(), q.options()), dkv = at::empty(kv.sizes(), kv.options());
-  if (q.numel() == 0 || kv.numel() == 0) return {dq.zero_(), dkv.zero_()};
+  auto dq = at::empty(q.sizes(), q.options());
+  at::Tensor dkv = want_kv ? at::empty(kv.sizes(), kv.options()) : at::Tensor();
+  if (q.numel() == 0 || kv.numel() == 0) return {dq.zero_(), want_kv ? dkv.zero_() : dkv};
   p.o = (const u16*)out.data_ptr();
   p.dout = (const u16*)dout.data_ptr();
   p.out = (u16*)dq.data_ptr();
-  p.dkv = (u16*)dkv.data_ptr();
+  p.dkv = want_kv ? (u16*)dkv.data_ptr() : nullptr;
   p.lse = lse.data_ptr<float>();
   by_type_and_width(p, q.scalar_type(), [&](auto e, auto dp) {
     typedef decltype(e) E;
@@ -1041,17 +1042,19 @@ std::vector<at::Tensor> cross_bwd(const at::Tensor& dout, const at::Tensor& q, c
     split_axis(pk, (int64_t)pk.blocks * p.B * p.N, p.M, RT);
     // one workspace: the rows' sums of dP, then the parts of split gradients
     const int64_t rows = ((int64_t)p.B * p.N * p.M + 7) / 8 * 8;
-    const int64_t nq = p.splits > 1 ? p.splits * p.out_numel : 0, nkv = pk.splits > 1 ? pk.splits * p.dkv_numel : 0;
+    const int64_t nq = p.splits > 1 ? p.splits * p.out_numel : 0, nkv = want_kv && pk.splits > 1 ? pk.splits * p.dkv_numel : 0;
     auto work = at::empty({rows + nq + nkv}, q.options().dtype(at::kFloat));
     p.delta = pk.delta = work.data_ptr<float>();
     p.part = p.delta + rows;
     pk.part = p.part + nq;
     hipLaunchKernelGGL((cross_dq_kernel<E, dp>), dim3(grid_of(p)), dim3(kThreads), 0, stream(), p);
     LAUNCH_CHECK();
-    hipLaunchKernelGGL((cross_dkv_kernel<E, dp, RT>), dim3(grid_of(pk)), dim3(kThreads), 0, stream(), pk);
-    LAUNCH_CHECK();
+    if (want_kv) {
+      hipLaunchKernelGGL((cross_dkv_kernel<E, dp, RT>), dim3(grid_of(pk)), dim3(kThreads), 0, stream(), pk);
+      LAUNCH_CHECK();
+    }
     auto job = [](const CrossParams& c, u16* to, int64_t n) {
-      return PartSum{c.part, to, n, c.splits, c.splits > 1 ? up(n, 8 * kThreads) : 0};
+      return PartSum{c.part, to, n, c.splits, to && c.splits > 1 ? up(n, 8 * kThreads) : 0};
     };
     const PartSum a = job(p, p.out, p.out_numel), b = job(pk, pk.dkv, pk.dkv_numel);
     if (a.blocks + b.blocks > 0) {
@@ -1094,7 +1097,8 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
     if (s[4].defined()) lengths = s[4];
     auto g = grads[0].contiguous();
     if (reinterpret_cast<uintptr_t>(g.data_ptr()) % 16) g = g.clone();
-    auto d = cross_bwd(g, s[0], s[1], s[2], s[3], lengths, ctx->saved_data["scale"].toDouble());
+    // frozen states: no dK and dV (dQ's kernel always runs, it has the row sums)
+    auto d = cross_bwd(g, s[0], s[1], s[2], s[3], lengths, ctx->saved_data["scale"].toDouble(), ctx->needs_input_grad(1));
     return {d[0], d[1], at::Tensor(), at::Tensor()};
   }
 };

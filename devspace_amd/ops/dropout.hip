@@ -126,11 +126,12 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const typename E::S* 
 
 // ------------------------------------------------------------------------------ dropout + add + norm
 
-// Sum over the lanes that share a row: a wave, or the block's four waves through LDS.
+// Sum over the lanes that share a row: part of a wave, a wave, or the block's four waves through LDS.
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-  v = wave_sum(v);
-  if (LANES == 64) return v;
+#pragma unroll
+  for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if (LANES <= 64) return v;
   const int wave = threadIdx.x >> 6;
   __syncthreads();  // the last row's sums have been read
   if ((threadIdx.x & 63) == 0) red[wave] = v;
@@ -138,7 +139,7 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// LANES lanes per row (64 or 256), VPL groups of eight elements per lane: lane l owns groups l, l + LANES, ...
+// LANES lanes per row (4 to 64, or the block's 256), VPL groups of eight elements per lane: lane l owns groups l, l + LANES, ...
 // and keeps them in registers between the sum of squares and the scaled store, so that each tensor passes once.
 template <typename E, int LANES, int VPL>
 __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename E::S* __restrict__ x,
@@ -148,9 +149,9 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
                                                                  typename E::S* __restrict__ y, float* __restrict__ rstd,
                                                                  int64_t R, int D, float eps, Drop drop) {
   __shared__ float red[4];
-  const int lane = LANES == 64 ? threadIdx.x & 63 : threadIdx.x;
-  const int64_t row = LANES == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-  if (LANES == 64 && row >= R) return;
+  const int lane = threadIdx.x & (LANES - 1);
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  if (LANES < kThreads && row >= R) return;
   const Key key(drop);
   const int nvec = (D + 7) >> 3;
   const int64_t base = row * D;
@@ -193,18 +194,18 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
   }
 }
 
-// A block owns rows_per_block rows (with 64 lanes per row its four waves take turns); each lane adds the
-// weight gradient of its columns in registers, and the block writes one fp32 row of partial sums, which
-// col_sum_kernel adds in a fixed order.
+// A block owns rows_per_block rows (its groups of LANES lanes take turns); each lane adds the weight gradient of
+// its columns in registers, and the block writes one fp32 row of partial sums, which part_sum_kernel adds in a
+// fixed order.
 template <typename E, int LANES, int VPL>
 __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
     const typename E::S* __restrict__ dy, const typename E::S* __restrict__ ds, const typename E::S* __restrict__ s,
     const typename E::S* __restrict__ w, const float* __restrict__ rstd, typename E::S* __restrict__ dx,
     typename E::S* __restrict__ dd, float* __restrict__ part, int64_t R, int D, int rows_per_block, Drop drop) {
   __shared__ float red[4];
-  extern __shared__ float sdw[];  // [4][D], with 64 lanes per row
-  const int lane = LANES == 64 ? threadIdx.x & 63 : threadIdx.x;
-  constexpr int kStep = LANES == 64 ? 4 : 1;
+  constexpr int kStep = kThreads / LANES;  // groups
+  extern __shared__ float sdw[];           // [kStep][D], with more than one
+  const int lane = threadIdx.x & (LANES - 1);
   const Key key(drop);
   const int nvec = (D + 7) >> 3;
   float acc[VPL][8];
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
 #pragma unroll
     for (int k = 0; k < VPL; ++k) load8<E>(w + 8 * (lane + LANES * k), D - 8 * (lane + LANES * k), wv[k]);
   }
-  for (int64_t row = r0 + (LANES == 64 ? threadIdx.x >> 6 : 0); row < r1; row += kStep) {
+  for (int64_t row = r0 + threadIdx.x / LANES; row < r1; row += kStep) {
     const int64_t base = row * D;
     float g[VPL][8], sv[VPL][8];
     float dot = 0.f;
@@ -260,8 +261,8 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
     }
   }
   float* out = part + (int64_t)blockIdx.x * D;
-  if (LANES == 64) {
-    float* mine = sdw + (threadIdx.x >> 6) * D;
+  if (LANES < kThreads) {
+    float* mine = sdw + threadIdx.x / LANES * D;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
       const int i = lane + LANES * k;
@@ -270,7 +271,12 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
         if (8 * i + j < D) mine[8 * i + j] = acc[k][j];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < D; c += kThreads) out[c] = (sdw[c] + sdw[D + c]) + (sdw[2 * D + c] + sdw[3 * D + c]);
+    for (int c = threadIdx.x; c < D; c += kThreads) {
+      float t = 0.f;
+#pragma unroll
+      for (int g = 0; g < kStep; ++g) t += sdw[g * D + c];
+      out[c] = t;
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
@@ -370,13 +376,16 @@ at::Tensor dropout_apply(const at::Tensor& d, const at::Tensor& x, const Drop& d
   return y;
 }
 
-// Lanes per row and groups per lane of the norm kernels: a wave per row up to 2048 columns (no barrier, four
-// rows in flight per block), the whole block beyond.
+// Lanes per row and groups per lane of the norm kernels: as many lanes as a narrow row has groups (several rows
+// per wave: 4128008 rows x 22 forward and backward take 1 wave per row 8709 us), a wave per row up to 2048 columns
+// (no barrier, four rows in flight per block), the whole block beyond.
 template <typename F>
 void by_width(int64_t D, F&& f) {
   using std::integral_constant;
   const int64_t n = (D + 7) / 8;
-  if (n <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  if (n <= 4) f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else if (n <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (n <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (n <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
   else if (n <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
   else if (n <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
@@ -397,7 +406,7 @@ NormForward drop_norm_fwd(const at::Tensor& x, const at::Tensor& delta, const at
     typedef decltype(e) E;
     typedef typename E::S S;
     by_width(D, [&](auto lanes, auto vpl) {
-      const int64_t blocks = lanes == 64 ? (R + 3) / 4 : R;
+      const int64_t at_once = kThreads / lanes, blocks = (R + at_once - 1) / at_once;
       TORCH_CHECK(blocks < (1ll << 31), "dropout_add_rms_norm: too many rows");
       hipLaunchKernelGGL((drop_norm_fwd_kernel<E, lanes, vpl>), dim3((unsigned)blocks), dim3(kThreads), 0, stream(),
                          (const S*)x.data_ptr(), (const S*)delta.data_ptr(), (const S*)w.data_ptr(), (S*)o.sum.data_ptr(),
@@ -419,14 +428,14 @@ std::vector<at::Tensor> drop_norm_bwd(const at::Tensor& dy, const at::Tensor& ds
     typedef decltype(e) E;
     typedef typename E::S S;
     by_width(D, [&](auto lanes, auto vpl) {
-      // two rows per wave, or per block; at most 1024 rows of partial sums
-      const int64_t at_once = lanes == 64 ? 4 : 1;
+      // two rows per group of lanes; at most 1024 rows of partial sums
+      const int64_t at_once = kThreads / lanes;
       const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(1024, (R + 2 * at_once - 1) / (2 * at_once)));
       const int64_t per = (R + blocks - 1) / blocks;
       TORCH_CHECK(per < (1ll << 31), "dropout_add_rms_norm: too many rows");
       auto part = at::empty({blocks, D}, s.options().dtype(at::kFloat));
       hipLaunchKernelGGL((drop_norm_bwd_kernel<E, lanes, vpl>), dim3((unsigned)blocks), dim3(kThreads),
-                         lanes == 64 ? 4 * D * sizeof(float) : 0, stream(), dy.defined() ? (const S*)dy.data_ptr() : nullptr,
+                         at_once > 1 ? at_once * D * sizeof(float) : 0, stream(), dy.defined() ? (const S*)dy.data_ptr() : nullptr,
                          ds.defined() ? (const S*)ds.data_ptr() : nullptr, (const S*)s.data_ptr(), (const S*)w.data_ptr(),
                          rstd.data_ptr<float>(), (S*)dx.data_ptr(), (S*)dd.data_ptr(), part.data_ptr<float>(), R, (int)D,
                          (int)per, drop);

@@ -368,7 +368,9 @@ class Rotary(nn.Module):
 # ------------------------------------------------------------------------------ dropout
 
 
-def _check_dropout(op, p, seed, offset):
+def _check_dropout(op, p, seed, offset, dtype=torch.float32):
+    if not dtype.is_floating_point:
+        raise ValueError(f"{op}: floating-point data wanted")
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"{op}: p must be within 0 and 1")
     if not 0 <= offset < 1 << 32:
@@ -415,7 +417,7 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
     seed: a whole number of 64 bits, or a tensor of one int64 on the data's device (a captured graph
     reads it anew at each replay; it must not change between a forward pass and its backward pass).
     offset: 0 to 2^32 - 1, to tell the dropouts of one step apart. The masks are the same on every device."""
-    seed, at = _check_dropout("dropout", p, seed, offset)
+    seed, at = _check_dropout("dropout", p, seed, offset, x.dtype)
     if x.is_cuda and x.dtype in _HIP_FLOATS:
         return ext().dropout(x, None, float(p), seed, at, offset)
     return _dropped(x, p, seed, at, offset).to(x.dtype)
@@ -423,7 +425,7 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
 
 def dropout_add(x: torch.Tensor, delta: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
     """x + dropout(delta, p, seed, offset) in one kernel, rounded once."""
-    seed, at = _check_dropout("dropout_add", p, seed, offset)
+    seed, at = _check_dropout("dropout_add", p, seed, offset, x.dtype)
     if x.shape != delta.shape or x.dtype != delta.dtype or x.device != delta.device:
         raise ValueError("dropout_add: x and delta must agree in shape, type and device")
     if x.is_cuda and x.dtype in _HIP_FLOATS:
@@ -435,8 +437,9 @@ def dropout_add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Ten
                          eps: float | None = None, offset: int = 0):
     """add_rms_norm() of a residual stream with dropout: returns (s, y) with
     s = x + dropout(delta, p, seed, offset) and y = rms_norm(s) * weight, one kernel each way (and a
-    small one for the weight's gradient). y is made of the sum before it is rounded to s."""
-    seed, at = _check_dropout("dropout_add_rms_norm", p, seed, offset)
+    small one for the weight's gradient). y is made of the sum before it is rounded to s. On a GPU rows
+    (the last dimension) of up to 16384 elements."""
+    seed, at = _check_dropout("dropout_add_rms_norm", p, seed, offset, x.dtype)
     if x.shape != delta.shape or x.dtype != delta.dtype or x.device != delta.device:
         raise ValueError("dropout_add_rms_norm: x and delta must agree in shape, type and device")
     if x.dim() < 1 or weight.shape != x.shape[-1:] or weight.dtype != x.dtype:
@@ -451,7 +454,8 @@ def dropout_add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Ten
 
 class Dropout(nn.Module):
     """nn.Dropout(p) on the fused kernels. Each call takes its seed from PyTorch's CPU generator (so
-    torch.manual_seed and checkpointed recomputation repeat it); `residual` is added in the same kernel."""
+    torch.manual_seed and checkpointed recomputation repeat it); `residual` is added in the same kernel.
+    A captured graph keeps the seeds of its capture: inside one, call dropout() with a seed tensor."""
 
     def __init__(self, p: float = 0.5):
         super().__init__()

@@ -36,16 +36,82 @@ struct RotaryParams {
   int64_t tokens;  // B * T
   int nseg, D, R, T;
   int tokens_per_block, per_token, per_head;  // work items: of a token, of a head
+  int turned, pad;                            // a head's items of turned pairs; floats of a token's cosines in LDS
   FastDiv by_token, by_head, by_T, by_half;
   float magnitude, sign;
   bool pos64;
 };
 
-// One work item: V pairs of one head of one token, or 2 V columns to copy.
+// n values from LDS at 4 x N bytes' alignment
+template <int N>
+__device__ __forceinline__ void lds_floats(const float* p, float (&v)[N]) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + i);
+      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = p[i];
+  }
+}
+
+// The W pairs of a head from `pair` on, their cosines and sines at cs and sn.
+template <typename E, int W, bool INTERLEAVED>
+__device__ __forceinline__ void turn(const typename E::S* in, typename E::S* out, int pair, int half, const float* cs,
+                                     const float* sn) {
+  typedef typename E::S S;
+  float c[W], s[W];
+  lds_floats(cs, c);
+  lds_floats(sn, s);
+  if (INTERLEAVED) {
+    auto x = load_pack<S, 2 * W>(in + 2 * pair);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float a = E::get(x.v[2 * i]), b = E::get(x.v[2 * i + 1]);
+      x.v[2 * i] = E::put(a * c[i] - b * s[i]);
+      x.v[2 * i + 1] = E::put(a * s[i] + b * c[i]);
+    }
+    store_pack<S, 2 * W>(out + 2 * pair, x);
+  } else {
+    auto x = load_pack<S, W>(in + pair), y = load_pack<S, W>(in + half + pair);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float a = E::get(x.v[i]), b = E::get(y.v[i]);
+      x.v[i] = E::put(a * c[i] - b * s[i]);
+      y.v[i] = E::put(a * s[i] + b * c[i]);
+    }
+    store_pack<S, W>(out + pair, x);
+    store_pack<S, W>(out + half + pair, y);
+  }
+}
+
+// The last n < 2 W pairs (or columns to copy) in pieces of W, W / 2, ... 1.
+template <typename E, int W, bool INTERLEAVED>
+__device__ __forceinline__ void turn_rest(const typename E::S* in, typename E::S* out, int pair, int half, const float* cs,
+                                          const float* sn) {
+  if ((half - pair) & W) {
+    turn<E, W, INTERLEAVED>(in, out, pair, half, cs, sn);
+    pair += W, cs += W, sn += W;
+  }
+  if constexpr (W > 1) turn_rest<E, W / 2, INTERLEAVED>(in, out, pair, half, cs, sn);
+}
+template <typename S, int W>
+__device__ __forceinline__ void copy_rest(const S* in, S* out, int n) {
+  if (n & W) {
+    store_pack<S, W>(out, load_pack<S, W>(in));
+    in += W, out += W;
+  }
+  if constexpr (W > 1) copy_rest<S, W / 2>(in, out, n);
+}
+
+// One work item: V pairs of one head of one token, or 2 V columns to copy; the last item of either kind may have
+// fewer.
 template <typename E, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
   typedef typename E::S S;
-  extern __shared__ float lds[];  // [tokens][cos R/2 | sin R/2]
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // [tokens][cos | sin], each padded to p.pad
   const int half = p.R >> 1;
   const int64_t token0 = (int64_t)blockIdx.x * p.tokens_per_block;
   const int n = (int)min((int64_t)p.tokens_per_block, p.tokens - token0);
@@ -64,8 +130,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
     const double turns = x * (p.freq[i] * 0.15915494309189533577);
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-    lds[j * p.R + i] = c * p.magnitude;
-    lds[j * p.R + half + i] = s * p.magnitude * p.sign;
+    lds[2 * j * p.pad + i] = c * p.magnitude;
+    lds[(2 * j + 1) * p.pad + i] = s * p.magnitude * p.sign;
   }
   __syncthreads();
   const unsigned items = (unsigned)n * p.per_token;
@@ -82,35 +148,14 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
     S* out = static_cast<S*>(sg.out) + b * sg.ob + t * sg.ot + h * sg.oh;
     const int pair = (int)item * V;
     if (sg.turn && pair < half) {
-      const float* cs = lds + j * p.R + pair;
-      const float* sn = cs + half;
-      if (INTERLEAVED) {
-        auto x = load_pack<S, 2 * V>(in + 2 * pair);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float a = E::get(x.v[2 * i]), bb = E::get(x.v[2 * i + 1]);
-          x.v[2 * i] = E::put(a * cs[i] - bb * sn[i]);
-          x.v[2 * i + 1] = E::put(a * sn[i] + bb * cs[i]);
-        }
-        store_pack<S, 2 * V>(out + 2 * pair, x);
-      } else {
-        auto x = load_pack<S, V>(in + pair), y = load_pack<S, V>(in + half + pair);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float a = E::get(x.v[i]), bb = E::get(y.v[i]);
-          x.v[i] = E::put(a * cs[i] - bb * sn[i]);
-          y.v[i] = E::put(a * sn[i] + bb * cs[i]);
-        }
-        store_pack<S, V>(out + pair, x);
-        store_pack<S, V>(out + half + pair, y);
-      }
+      const float* cs = lds + 2 * j * p.pad + pair;
+      const float* sn = cs + p.pad;
+      if (pair + V <= half) turn<E, V, INTERLEAVED>(in, out, pair, half, cs, sn);
+      else if constexpr (V > 1) turn_rest<E, V / 2, INTERLEAVED>(in, out, pair, half, cs, sn);
     } else {
-      const int c = 2 * pair;  // the R turned columns come first, then the copied ones
-      if (c + 2 * V <= p.D) {
-        store_pack<S, 2 * V>(out + c, load_pack<S, 2 * V>(in + c));
-      } else {
-        for (int i = c; i < p.D; ++i) out[i] = in[i];
-      }
+      const int c = sg.turn ? p.R + 2 * (pair - p.turned * V) : 2 * pair;
+      if (c + 2 * V <= p.D) store_pack<S, 2 * V>(out + c, load_pack<S, 2 * V>(in + c));
+      else if (c < p.D) copy_rest<S, V>(in + c, out + c, p.D - c);
     }
   }
 }
@@ -126,19 +171,22 @@ void check_positions(const c10::optional<at::Tensor>& pos, int64_t B, int64_t T,
 
 template <typename E>
 void launch_rotary(RotaryParams& p, bool interleaved, hipStream_t st) {
-  // the widest access of up to 16 bytes whose pairs divide the half
+  // accesses of 16 bytes; of the half's size where that is less
   constexpr int kWide = 16 / (int)sizeof(typename E::S);
   const int half = p.R / 2;
   int v = kWide;
-  while (half % v) v /= 2;
-  p.per_head = (p.D + 2 * v - 1) / (2 * v);
+  while (v > half) v /= 2;
+  p.turned = (half + v - 1) / v;
+  // a head's items: its turned pairs, then its copied columns; a copied head needs no more than that
+  p.per_head = std::max(p.turned + (p.D - p.R + 2 * v - 1) / (2 * v), (p.D + 2 * v - 1) / (2 * v));
+  p.pad = (half + 3) / 4 * 4;
   int heads = 0;
   for (int i = 0; i < p.nseg; ++i) heads += p.seg[i].heads;
   TORCH_CHECK((int64_t)heads * p.per_head * kMaxTokens < (1ll << 31), "rotary: too many heads");
   p.per_token = heads * p.per_head;
   // about four items per thread, so that the sines' latency is shared, but not fewer blocks than CUs
   int tb = std::max(1, std::min(kMaxTokens, 4 * kThreads / std::max(1, p.per_token)));
-  while (tb > 1 && ((p.tokens + tb - 1) / tb < 512 || tb * p.R * 4 > 32768)) tb /= 2;
+  while (tb > 1 && ((p.tokens + tb - 1) / tb < 512 || tb * p.pad * 8 > 32768)) tb /= 2;
   p.tokens_per_block = tb;
   p.by_token = FastDiv((unsigned)p.per_token);
   p.by_head = FastDiv((unsigned)p.per_head);
@@ -146,7 +194,7 @@ void launch_rotary(RotaryParams& p, bool interleaved, hipStream_t st) {
   p.by_half = FastDiv((unsigned)half);
   const int64_t blocks = (p.tokens + tb - 1) / tb;
   TORCH_CHECK(blocks < (1ll << 31), "rotary: too many tokens");
-  const size_t lds = (size_t)tb * p.R * sizeof(float);
+  const size_t lds = (size_t)tb * 2 * p.pad * sizeof(float);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), lds, st, p); };
 #define ROTARY_CASE(W)                                                                        \
   case W:                                                                                     \
@@ -251,6 +299,7 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
     ctx->saved_data["packed"] = packed;
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["magnitude"] = magnitude;
+    ctx->set_materialize_grads(false);  // a tensor whose result was not used costs nothing
     std::vector<at::Tensor> xs{q};
     if (k) xs.push_back(*k);
     return rotary_apply(std::move(xs), packed, pos, start, freq, interleaved, magnitude, false);

@@ -143,6 +143,10 @@ CASES = [  # dtype, B, Tq, Tk, H, G, D, lengths
     ("bf16", 4, 64, 512, 4, 1, 64, (512, 1, 300, 449)),
     ("bf16", 1, 2000, 31, 2, 1, 104, None),
     ("fp16", 1, 3, 2000, 2, 1, 16, (1999,)),
+    ("fp16", 2, 40, 2, 4, 1, 64, None),  # few states: dO . O nearly equals dP
+    ("bf16", 1, 1000, 3000, 1, 1, 64, None),  # both axes split
+    ("bf16", 1, 200, 900, 14, 7, 128, (899,)),  # tiles that begin inside a token's group of heads
+    ("fp16", 2, 31, 64, 5, 5, 88, (64, 63)),
 ]
 
 
@@ -159,6 +163,16 @@ def test_forward_and_backward(dtype, b, tq, tk, h, g, d, lengths):
         assert torch.equal(got[k], again[k]), k
     with torch.no_grad():
         assert torch.equal(fused.cross_attention(q, kv, n), got["o"])
+
+
+@gpu
+def test_frozen_states_and_frozen_queries():
+    dev = _cuda()
+    q, kv, do = _inputs(dev, torch.bfloat16, 2, 50, 1000, 4, 2, 64)
+    want = _run(q, kv, do, None)
+    (dq,) = torch.autograd.grad(fused.cross_attention(q, kv.detach()), q, do)
+    (dkv,) = torch.autograd.grad(fused.cross_attention(q.detach(), kv), kv, do)
+    assert torch.equal(dq, want["dq"]) and torch.equal(dkv, want["dkv"])
 
 
 @gpu

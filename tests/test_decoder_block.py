@@ -1,0 +1,104 @@
+"""Rotary positions, dropout and cross attention together with the framework's attention, norm and SwiGLU: a decoder
+block over an encoder's states, trained, and one token of it as when sampling."""
+import pytest
+import torch
+
+from devspace_amd.ops import fused
+
+gpu = pytest.mark.gpu
+B, T, S, H, D = 2, 128, 90, 4, 64
+DIM = H * D
+P, SEED = 0.1, 1234
+
+
+def _weights(dtype, device):
+    gen = torch.Generator().manual_seed(0)
+    shapes = dict(qkv=(3 * DIM, DIM), proj=(DIM, DIM), q=(DIM, DIM), kv=(2 * DIM, DIM), out=(DIM, DIM), up=(4 * DIM, DIM),
+                  down=(DIM, 2 * DIM))
+    w = {k: torch.randn(s, generator=gen) * s[1] ** -0.5 for k, s in shapes.items()}
+    w.update({f"norm{i}": 1 + 0.1 * torch.randn(DIM, generator=gen) for i in range(3)})
+    # both sides compute with the same (bf16) values
+    return {k: v.bfloat16().to(dtype).to(device).requires_grad_() for k, v in w.items()}
+
+
+def _block(w, x, states, lengths, freqs, p=P, start=0):
+    b, t, _ = x.shape
+    h = fused.rms_norm(x, w["norm0"], 1e-5)
+    qkv = fused.rotary_qkv((h @ w["qkv"].T).view(b, t, 3, H, D), start, freqs)
+    a = fused.attention(qkv, causal=True).reshape(b, t, DIM)
+    x, h = fused.dropout_add_rms_norm(x, a @ w["proj"].T, w["norm1"], p, SEED, eps=1e-5, offset=0)
+    kv = (states @ w["kv"].T).view(b, -1, 2, H, D)
+    c = fused.cross_attention((h @ w["q"].T).view(b, t, H, D), kv, lengths).reshape(b, t, DIM)
+    x, h = fused.dropout_add_rms_norm(x, c @ w["out"].T, w["norm2"], p, SEED, eps=1e-5, offset=1)
+    return fused.dropout_add(x, fused.swiglu(h @ w["up"].T) @ w["down"].T, p, SEED, offset=2)
+
+
+def _inputs(dtype, device):
+    gen = torch.Generator().manual_seed(1)
+    x, states, g = (torch.randn(s, generator=gen).bfloat16() for s in ((B, T, DIM), (B, S, DIM), (B, T, DIM)))
+    return (x.to(dtype).to(device).requires_grad_(), states.to(dtype).to(device).requires_grad_(), g.to(dtype).to(device),
+            torch.tensor([S, 37], device=device), fused.rotary_frequencies(D, device=device)[0])
+
+
+def _train(dtype, device):
+    w = _weights(dtype, device)
+    x, states, g, lengths, freqs = _inputs(dtype, device)
+    y = _block(w, x, states, lengths, freqs)
+    leaves = {"x": x, "states": states, **w}
+    grads = torch.autograd.grad(y, list(leaves.values()), g)
+    return {"y": y, **{"d" + k: v for k, v in zip(leaves, grads)}}
+
+
+def _off(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).norm() / b.norm())
+
+
+def test_block_runs_on_cpu_and_drops():
+    got = _train(torch.float64, "cpu")
+    assert all(v.isfinite().all() for v in got.values())
+    w = _weights(torch.float64, "cpu")
+    x, states, _, lengths, freqs = _inputs(torch.float64, "cpu")
+    assert _off(_block(w, x, states, lengths, freqs, p=0.0), got["y"]) > 0.01  # the dropouts matter
+    moved = _block(w, x, states, lengths, freqs, start=77)  # a shift of all positions changes nothing
+    torch.testing.assert_close(moved, got["y"], atol=1e-9, rtol=0)
+
+
+@gpu
+def test_block_trains_like_64_bits():
+    """14 tensors are rounded to bf16 on the way forward and about twice as many on the way back. A rounding is off by
+    2^-8 of an element at the most, so by 2^-8 in the norm; each step is passed on by a norm of about one (norms,
+    products with random matrices of that norm, softmax averages), so 42 of them bound the relative error."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    fused.ext()
+    got, want = _train(torch.bfloat16, "cuda"), _train(torch.float64, "cpu")
+    for k in want:
+        assert got[k].dtype == torch.bfloat16 and got[k].shape == want[k].shape
+        steps = 14 if k == "y" else 42
+        assert _off(got[k], want[k]) < steps * 2.0 ** -8, (k, _off(got[k], want[k]))
+
+
+@gpu
+def test_one_token_is_a_row_of_the_sequence():
+    """Serving: the same token alone, its keys already turned at their own positions."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    fused.ext()
+    torch.manual_seed(2)
+    dev = "cuda"
+    freqs = fused.rotary_frequencies(D, device=dev)[0]
+    q, k = torch.randn(B, T, H, D, device=dev).bfloat16(), torch.randn(B, T, 1, D, device=dev).bfloat16()
+    kv = torch.randn(B, S, 2, 2, D, device=dev).bfloat16()
+    lengths = torch.tensor([S, 37], device=dev)
+    with torch.no_grad():
+        tq, tk = fused.rotary_qk(q, k, 1000, freqs)
+        o = fused.cross_attention(tq, kv, lengths)
+        for t in (0, 57, T - 1):
+            at = torch.full((B, 1), 1000 + t, device=dev)
+            one_q, one_k = fused.rotary_qk(q[:, t:t + 1], k[:, t:t + 1], at, freqs)
+            assert torch.equal(one_q, tq[:, t:t + 1]) and torch.equal(one_k, tk[:, t:t + 1])
+            one = fused.cross_attention(one_q, kv, lengths)
+            # two kernels with the same roundings in another order: probabilities 2^-8 each, the outputs too
+            size = kv[:, :, 1].float().abs().amax()
+            assert ((one - o[:, t:t + 1]).abs() <= 4 * 2.0 ** -8 * size).all()

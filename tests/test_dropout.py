@@ -100,7 +100,7 @@ def test_kept_share():
 
 def test_refusals_cpu():
     x, w = torch.randn(2, 4), torch.randn(4)
-    for call in (lambda: fused.dropout(x, -0.1, 0), lambda: fused.dropout(x, 1.1, 0), lambda: fused.dropout(x, 0.1, 1 << 64),
+    for call in (lambda: fused.dropout(x.long(), 0.1, 0), lambda: fused.dropout(x, -0.1, 0), lambda: fused.dropout(x, 1.1, 0), lambda: fused.dropout(x, 0.1, 1 << 64),
                  lambda: fused.dropout(x, 0.1, 0, offset=1 << 32), lambda: fused.dropout(x, 0.1, torch.zeros(2).long()),
                  lambda: fused.dropout(x, float("nan"), 0), lambda: fused.dropout_add(x, x[:1], 0.1, 0),
                  lambda: fused.dropout_add(x, x.double(), 0.1, 0), lambda: fused.dropout_add_rms_norm(x, x, w[:2], 0.1, 0),
@@ -151,7 +151,7 @@ def test_dropout_and_add_forward_and_backward(dtype, shape, p):
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,dim", [(1, 1), (3, 24), (37, 768), (64, 1023), (5, 2048), (9, 2051), (6, 4096), (3, 8191), (2, 16384),
-                                      (4097, 64)])
+                                      (4097, 64), (20003, 22), (777, 100), (301, 130)])
 @pytest.mark.parametrize("use", ["both", "y", "s"])
 def test_dropout_add_rms_norm_forward_and_backward(dtype, rows, dim, use):
     dev, dt = _cuda(), DTYPES[dtype]
@@ -260,7 +260,8 @@ def test_captured_step_reads_its_seed_at_each_replay():
     def step():
         s, y = fused.dropout_add_rms_norm(x, d, w, 0.3, seed, offset=2)
         z = fused.dropout(y, 0.5, seed)
-        return [s, y, z, *torch.autograd.grad((s, z), (x, d, w), (gs, gy))]
+        grads = torch.autograd.grad((s, z), (x, d, w), (gs, gy))
+        return [s.detach(), y.detach(), z.detach(), *grads]
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

@@ -110,6 +110,9 @@ CASES = [  # dtype, B, T, H, N, D, R, interleaved, scaling
     ("bf16", 1, 1, 1, 1, 2, 2, False, "none"),
     ("fp32", 4, 700, 8, 1, 64, 64, True, "none"),
     ("bf16", 1, 4, 33, 31, 256, 256, True, "none"),
+    ("bf16", 2, 21, 3, 2, 128, 66, True, "yarn"),  # 33 pairs and 62 copied columns: neither a whole number of accesses
+    ("fp16", 2, 21, 3, 2, 127, 66, False, "none"),
+    ("fp32", 1, 40, 2, 2, 99, 46, False, "linear"),
 ]
 
 

@@ -133,7 +133,42 @@ def op_cases(dev):
         y_ = F.rms_norm(s_, (D,), w, eps)
         torch.autograd.backward([s_, y_], [dy, dy])
 
+    freqs, _ = fused.rotary_frequencies(64, device=dev)
+    angle = torch.arange(512, device=dev)[:, None] * freqs
+    cos, sin = (f.to(torch.bfloat16)[:, None, None] for f in (angle.cos(), angle.sin()))  # an eager model's table
+    dqkv = torch.randn_like(qkv)
+
+    def rotary_fused():
+        fused.rotary_qkv(qkv, None, freqs).backward(dqkv)
+
+    def rotary_eager():
+        a, b = qkv[:, :, :2].chunk(2, -1)
+        torch.cat((torch.cat((a * cos - b * sin, a * sin + b * cos), -1), qkv[:, :, 2:]), 2).backward(dqkv)
+
+    def dropnorm_fused():
+        s_, y_ = fused.dropout_add_rms_norm(x, xd, w, 0.1, 7, eps)
+        torch.autograd.backward([s_, y_], [dy, dy])
+
+    def dropnorm_eager():
+        s_ = x + F.dropout(xd, 0.1)
+        y_ = F.rms_norm(s_, (D,), w, eps)
+        torch.autograd.backward([s_, y_], [dy, dy])
+
+    cq = torch.randn(8, 512, 16, 64, device=dev).bfloat16().requires_grad_()
+    ckv = torch.randn(8, 512, 2, 16, 64, device=dev).bfloat16().requires_grad_()
+
+    def cross_fused():
+        fused.cross_attention(cq, ckv).backward(dattn)
+
+    def cross_eager():
+        k, v = ckv.unbind(2)
+        o = F.scaled_dot_product_attention(cq.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
+        o.transpose(1, 2).reshape(8, 512, 1024).backward(dattn.view(8, 512, 1024))
+
     return {"attention fwd+bwd [8x512, 16 heads x 64]": (attn_fused, attn_eager),
+            "cross attention fwd+bwd [8x512 over 512, 16 heads x 64]": (cross_fused, cross_eager),
+            "rotary qkv fwd+bwd [8x512, 16 heads x 64]": (rotary_fused, rotary_eager),
+            "dropout + add + rmsnorm fwd+bwd [4096x1024]": (dropnorm_fused, dropnorm_eager),
             "residual add + rmsnorm fwd+bwd [4096x1024]": (addnorm_fused, addnorm_eager),
             "adamw step [67M bf16 params]": (opt_f.step, opt_e.step),
             "rmsnorm fwd+bwd [4096x1024]": (rms_fused, rms_eager),
@@ -203,13 +238,13 @@ def main():
         if None not in gf and None not in ge:
             graph[k] = (statistics.median(gf), statistics.median(ge))
     out = {}
-    print(f"{'case':42s} {'fused_us':>10} {'eager_us':>10} {'speedup':>8}   {'graph: fused_us':>15} {'eager_us':>9} "
+    print(f"{'case':56s} {'fused_us':>10} {'eager_us':>10} {'speedup':>8}   {'graph: fused_us':>15} {'eager_us':>9} "
           f"{'speedup':>8}   (medians, interleaved rounds)")
     for k, v in res.items():
         fm, em = statistics.median(v["fused"]), statistics.median(v["eager"])
         out[k] = {"fused_us": round(fm, 1), "eager_us": round(em, 1), "speedup": round(em / fm, 3),
                   "fused_min_us": round(min(v["fused"]), 1), "eager_min_us": round(min(v["eager"]), 1)}
-        line = f"{k:42s} {fm:>10.1f} {em:>10.1f} {em / fm:>8.2f}x"
+        line = f"{k:56s} {fm:>10.1f} {em:>10.1f} {em / fm:>8.2f}x"
         if k in graph:
             gfm, gem = graph[k]
             out[k].update({"graph_fused_us": round(gfm, 1), "graph_eager_us": round(gem, 1),

@@ -147,6 +147,7 @@ CASES = [  # dtype, B, Tq, Tk, H, G, D, lengths
     ("bf16", 1, 1000, 3000, 1, 1, 64, None),  # both axes split
     ("bf16", 1, 200, 900, 14, 7, 128, (899,)),  # tiles that begin inside a token's group of heads
     ("fp16", 2, 31, 64, 5, 5, 88, (64, 63)),
+    ("bf16", 3, 800, 1500, 2, 1, 64, (1500, 0, 600)),  # many rows joined
 ]
 
 

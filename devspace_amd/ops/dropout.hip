@@ -71,36 +71,56 @@ __device__ __forceinline__ void drop8(float f[8], int64_t row, unsigned v, const
   }
 }
 
-// Up to eight elements of a row: one wide access, or the tail element by element.
-template <typename E>
-__device__ __forceinline__ void load8(const typename E::S* p, int n, float f[8]) {
-  if (n >= 8) {
-    const auto x = load_pack<typename E::S, 8>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = E::get(x.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? E::get(p[i]) : 0.f;
-  }
+// Up to eight elements of a row as they are stored, 0 behind its end: one wide access, or the row's last n in pieces
+// of four, two and one. EVEN: rows are whole groups of eight. They are widened where they are used, so that no load
+// waits for another's values.
+template <typename S, bool EVEN>
+__device__ __forceinline__ Pack<S, 8> load8(const S* p, int n) {
+  if (EVEN || n >= 8) return load_pack<S, 8>(p);
+  const bool four = n & 4, two = n & 2, one = n & 1;
+  const S zero = (S)0;
+  Pack<S, 4> a = {{zero, zero, zero, zero}};
+  Pack<S, 2> b = {{zero, zero}};
+  S c = zero;
+  if (four) a = load_pack<S, 4>(p);
+  if (two) b = load_pack<S, 2>(p + (n & 4));
+  if (one) c = p[n & 6];
+  Pack<S, 8> x;
+  x.v[0] = four ? a.v[0] : two ? b.v[0] : c;
+  x.v[1] = four ? a.v[1] : b.v[1];
+  x.v[2] = four ? a.v[2] : two ? c : zero;
+  x.v[3] = a.v[3];
+  x.v[4] = four ? (two ? b.v[0] : c) : zero;
+  x.v[5] = four ? b.v[1] : zero;
+  x.v[6] = four && two ? c : zero;
+  x.v[7] = zero;
+  return x;
 }
 template <typename E>
+__device__ __forceinline__ void widen(const Pack<typename E::S, 8>& x, float f[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = E::get(x.v[i]);
+}
+template <typename E, bool EVEN>
 __device__ __forceinline__ void store8(typename E::S* p, int n, const float f[8]) {
-  if (n >= 8) {
-    Pack<typename E::S, 8> x;
+  typedef typename E::S S;
+  Pack<S, 8> x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x.v[i] = E::put(f[i]);
-    store_pack<typename E::S, 8>(p, x);
+  for (int i = 0; i < 8; ++i) x.v[i] = E::put(f[i]);
+  if (EVEN || n >= 8) {
+    store_pack<S, 8>(p, x);
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = E::put(f[i]);
+    const bool four = n & 4, two = n & 2;
+    if (four) store_pack<S, 4>(p, Pack<S, 4>{{x.v[0], x.v[1], x.v[2], x.v[3]}});
+    if (two) store_pack<S, 2>(p + (n & 4), Pack<S, 2>{{four ? x.v[4] : x.v[0], four ? x.v[5] : x.v[1]}});
+    if (n & 1) p[n & 6] = four ? (two ? x.v[6] : x.v[4]) : (two ? x.v[2] : x.v[0]);
   }
 }
 
 // ------------------------------------------------------------------------------ dropout, dropout + add
 
 // y = [x +] drop(d). Eight elements per work item; a launch covers rows row0.. with fewer than 2^31 items.
-template <typename E, bool ADD>
+template <typename E, bool ADD, bool EVEN>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const typename E::S* __restrict__ d,
                                                            const typename E::S* __restrict__ x,
                                                            typename E::S* __restrict__ y, unsigned items, int64_t row0,
@@ -112,15 +132,18 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const typename E::S* 
     const int64_t row = row0 + r;
     const int64_t at = row * D + 8 * (int64_t)v;
     const int n = D - 8 * (int)v;
+    const auto rd = load8<typename E::S, EVEN>(d + at, n);
+    Pack<typename E::S, 8> rx;
+    if (ADD) rx = load8<typename E::S, EVEN>(x + at, n);
     float f[8], g[8];
-    load8<E>(d + at, n, f);
-    if (ADD) load8<E>(x + at, n, g);
+    widen<E>(rd, f);
+    if (ADD) widen<E>(rx, g);
     drop8(f, row, v, key);
     if (ADD) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] += g[i];
     }
-    store8<E>(y + at, n, f);
+    store8<E, EVEN>(y + at, n, f);
   }
 }
 
@@ -141,7 +164,7 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 
 // LANES lanes per row (4 to 64, or the block's 256), VPL groups of eight elements per lane: lane l owns groups l, l + LANES, ...
 // and keeps them in registers between the sum of squares and the scaled store, so that each tensor passes once.
-template <typename E, int LANES, int VPL>
+template <typename E, int LANES, int VPL, bool EVEN>
 __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename E::S* __restrict__ x,
                                                                  const typename E::S* __restrict__ delta,
                                                                  const typename E::S* __restrict__ w,
@@ -155,13 +178,17 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
   const Key key(drop);
   const int nvec = (D + 7) >> 3;
   const int64_t base = row * D;
-  float s[VPL][8], d[VPL][8];
+  // the weight is loaded with the row, not behind its sum, where the registers hold it
+  constexpr bool kEarly = VPL <= 4;
+  Pack<typename E::S, 8> rx[VPL], rd[VPL], rw[VPL];
+  float s[VPL][8];
 #pragma unroll
   for (int k = 0; k < VPL; ++k) {
     const int i = lane + LANES * k;
     if (i < nvec) {
-      load8<E>(x + base + 8 * i, D - 8 * i, s[k]);
-      load8<E>(delta + base + 8 * i, D - 8 * i, d[k]);
+      rx[k] = load8<typename E::S, EVEN>(x + base + 8 * i, D - 8 * i);
+      rd[k] = load8<typename E::S, EVEN>(delta + base + 8 * i, D - 8 * i);
+      if (kEarly) rw[k] = load8<typename E::S, EVEN>(w + 8 * i, D - 8 * i);
     }
   }
   float ss = 0.f;
@@ -169,13 +196,16 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
   for (int k = 0; k < VPL; ++k) {
     const int i = lane + LANES * k;
     if (i < nvec) {
-      drop8(d[k], row, i, key);
+      float d[8];
+      widen<E>(rx[k], s[k]);
+      widen<E>(rd[k], d);
+      drop8(d, row, i, key);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        s[k][j] += d[k][j];
+        s[k][j] += d[j];
         ss += s[k][j] * s[k][j];  // columns behind the row are 0
       }
-      store8<E>(sum + base + 8 * i, D - 8 * i, s[k]);
+      store8<E, EVEN>(sum + base + 8 * i, D - 8 * i, s[k]);
     }
   }
   ss = row_sum<LANES>(ss, red);
@@ -186,10 +216,11 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
     const int i = lane + LANES * k;
     if (i < nvec) {
       float wv[8];
-      load8<E>(w + 8 * i, D - 8 * i, wv);
+      if (!kEarly) rw[k] = load8<typename E::S, EVEN>(w + 8 * i, D - 8 * i);
+      widen<E>(rw[k], wv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[k][j] *= r * wv[j];
-      store8<E>(y + base + 8 * i, D - 8 * i, s[k]);
+      store8<E, EVEN>(y + base + 8 * i, D - 8 * i, s[k]);
     }
   }
 }
@@ -197,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
 // A block owns rows_per_block rows (its groups of LANES lanes take turns); each lane adds the weight gradient of
 // its columns in registers, and the block writes one fp32 row of partial sums, which part_sum_kernel adds in a
 // fixed order.
-template <typename E, int LANES, int VPL>
+template <typename E, int LANES, int VPL, bool EVEN>
 __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
     const typename E::S* __restrict__ dy, const typename E::S* __restrict__ ds, const typename E::S* __restrict__ s,
     const typename E::S* __restrict__ w, const float* __restrict__ rstd, typename E::S* __restrict__ dx,
@@ -218,10 +249,12 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
   // kept in registers where they fit beside the weight gradient: the weight over all rows, and the residual's
   // gradient from the row's first loads on
   constexpr bool kKeepW = VPL <= 2, kEarly = VPL <= 4;
-  float wv[VPL][8], rv[VPL][8];
+  typedef Pack<typename E::S, 8> Raw;
+  Raw rw[VPL], rr[VPL], rg[VPL], rs[VPL];
   if (kKeepW) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) load8<E>(w + 8 * (lane + LANES * k), D - 8 * (lane + LANES * k), wv[k]);
+    for (int k = 0; k < VPL; ++k)
+      if (lane + LANES * k < nvec) rw[k] = load8<typename E::S, EVEN>(w + 8 * (lane + LANES * k), D - 8 * (lane + LANES * k));
   }
   for (int64_t row = r0 + threadIdx.x / LANES; row < r1; row += kStep) {
     const int64_t base = row * D;
@@ -230,17 +263,26 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
     const float r = rstd[row];
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
-      const int i = lane + LANES * k;
+      const int i = lane + LANES * k, n = D - 8 * i;
       if (i < nvec) {
-        if (dy) load8<E>(dy + base + 8 * i, D - 8 * i, g[k]);
-        load8<E>(s + base + 8 * i, D - 8 * i, sv[k]);
-        if (kEarly && ds) load8<E>(ds + base + 8 * i, D - 8 * i, rv[k]);
-        if (!kKeepW) load8<E>(w + 8 * i, D - 8 * i, wv[k]);
+        if (dy) rg[k] = load8<typename E::S, EVEN>(dy + base + 8 * i, n);
+        rs[k] = load8<typename E::S, EVEN>(s + base + 8 * i, n);
+        if (kEarly && ds) rr[k] = load8<typename E::S, EVEN>(ds + base + 8 * i, n);
+        if (!kKeepW) rw[k] = load8<typename E::S, EVEN>(w + 8 * i, n);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      if (lane + LANES * k < nvec) {
+        float wv[8];
+        widen<E>(rg[k], g[k]);
+        widen<E>(rs[k], sv[k]);
+        widen<E>(rw[k], wv);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (!dy) g[k][j] = 0.f;
           acc[k][j] += g[k][j] * sv[k][j] * r;
-          g[k][j] *= wv[k][j];
+          g[k][j] *= wv[j];
           dot += g[k][j] * sv[k][j];
         }
       }
@@ -249,14 +291,16 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
     const float c = dot * r * r * r * inv_d;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
-      const int i = lane + LANES * k;
+      const int i = lane + LANES * k, n = D - 8 * i;
       if (i < nvec) {
-        if (!kEarly && ds) load8<E>(ds + base + 8 * i, D - 8 * i, rv[k]);
+        float rv[8];
+        if (!kEarly && ds) rr[k] = load8<typename E::S, EVEN>(ds + base + 8 * i, n);
+        widen<E>(rr[k], rv);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[k][j] = r * g[k][j] - sv[k][j] * c + (ds ? rv[k][j] : 0.f);
-        store8<E>(dx + base + 8 * i, D - 8 * i, g[k]);
+        for (int j = 0; j < 8; ++j) g[k][j] = r * g[k][j] - sv[k][j] * c + (ds ? rv[j] : 0.f);
+        store8<E, EVEN>(dx + base + 8 * i, n, g[k]);
         drop8(g[k], row, i, key);
-        store8<E>(dd + base + 8 * i, D - 8 * i, g[k]);
+        store8<E, EVEN>(dd + base + 8 * i, n, g[k]);
       }
     }
   }
@@ -281,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
       const int i = lane + LANES * k;
-      if (i < nvec) store8<FP32>(out + 8 * i, D - 8 * i, acc[k]);
+      if (i < nvec) store8<FP32, EVEN>(out + 8 * i, D - 8 * i, acc[k]);
     }
   }
 }
@@ -369,7 +413,8 @@ at::Tensor dropout_apply(const at::Tensor& d, const at::Tensor& x, const Drop& d
                            x.defined() ? (const S*)x.data_ptr() : nullptr, (S*)y.data_ptr(), (unsigned)items, r0, (int)D,
                            FastDiv((unsigned)nvec), drop);
       };
-      x.defined() ? go(dropout_kernel<E, true>) : go(dropout_kernel<E, false>);
+      if (D % 8 == 0) x.defined() ? go(dropout_kernel<E, true, true>) : go(dropout_kernel<E, false, true>);
+      else x.defined() ? go(dropout_kernel<E, true, false>) : go(dropout_kernel<E, false, false>);
     });
     LAUNCH_CHECK();
   }
@@ -380,8 +425,12 @@ at::Tensor dropout_apply(const at::Tensor& d, const at::Tensor& x, const Drop& d
 // per wave: 4128008 rows x 22 forward and backward take 1 wave per row 8709 us), a wave per row up to 2048 columns
 // (no barrier, four rows in flight per block), the whole block beyond.
 template <typename F>
-void by_width(int64_t D, F&& f) {
+void by_width(int64_t D, F&& g) {
   using std::integral_constant;
+  auto f = [&](auto lanes, auto vpl) {
+    if (D % 8 == 0) g(lanes, vpl, std::true_type{});
+    else g(lanes, vpl, std::false_type{});
+  };
   const int64_t n = (D + 7) / 8;
   if (n <= 4) f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
   else if (n <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
@@ -405,10 +454,10 @@ NormForward drop_norm_fwd(const at::Tensor& x, const at::Tensor& delta, const at
   by_type(x.scalar_type(), [&](auto e) {
     typedef decltype(e) E;
     typedef typename E::S S;
-    by_width(D, [&](auto lanes, auto vpl) {
+    by_width(D, [&](auto lanes, auto vpl, auto even) {
       const int64_t at_once = kThreads / lanes, blocks = (R + at_once - 1) / at_once;
       TORCH_CHECK(blocks < (1ll << 31), "dropout_add_rms_norm: too many rows");
-      hipLaunchKernelGGL((drop_norm_fwd_kernel<E, lanes, vpl>), dim3((unsigned)blocks), dim3(kThreads), 0, stream(),
+      hipLaunchKernelGGL((drop_norm_fwd_kernel<E, lanes, vpl, even>), dim3((unsigned)blocks), dim3(kThreads), 0, stream(),
                          (const S*)x.data_ptr(), (const S*)delta.data_ptr(), (const S*)w.data_ptr(), (S*)o.sum.data_ptr(),
                          (S*)o.y.data_ptr(), o.rstd.data_ptr<float>(), R, (int)D, (float)eps, drop);
     });
@@ -427,14 +476,14 @@ std::vector<at::Tensor> drop_norm_bwd(const at::Tensor& dy, const at::Tensor& ds
   by_type(s.scalar_type(), [&](auto e) {
     typedef decltype(e) E;
     typedef typename E::S S;
-    by_width(D, [&](auto lanes, auto vpl) {
+    by_width(D, [&](auto lanes, auto vpl, auto even) {
       // two rows per group of lanes; at most 1024 rows of partial sums
       const int64_t at_once = kThreads / lanes;
       const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(1024, (R + 2 * at_once - 1) / (2 * at_once)));
       const int64_t per = (R + blocks - 1) / blocks;
       TORCH_CHECK(per < (1ll << 31), "dropout_add_rms_norm: too many rows");
       auto part = at::empty({blocks, D}, s.options().dtype(at::kFloat));
-      hipLaunchKernelGGL((drop_norm_bwd_kernel<E, lanes, vpl>), dim3((unsigned)blocks), dim3(kThreads),
+      hipLaunchKernelGGL((drop_norm_bwd_kernel<E, lanes, vpl, even>), dim3((unsigned)blocks), dim3(kThreads),
                          at_once > 1 ? at_once * D * sizeof(float) : 0, stream(), dy.defined() ? (const S*)dy.data_ptr() : nullptr,
                          ds.defined() ? (const S*)ds.data_ptr() : nullptr, (const S*)s.data_ptr(), (const S*)w.data_ptr(),
                          rstd.data_ptr<float>(), (S*)dx.data_ptr(), (S*)dd.data_ptr(), part.data_ptr<float>(), R, (int)D,

@@ -7,10 +7,11 @@
 // There is no causal mask, so the G query heads that share a key head are stacked: row m = t G + g, M = G Tq
 // rows over one set of keys, each key and value read once for all of them. All products run on
 // v_mfma_f32_32x32x16 (bf16 or fp16 in, fp32 out); softmax statistics and sums are in fp32. P and dS are
-// rounded to the 16-bit type as operands of the next product (half a step each, averaged over the keys),
-// as are the outputs; nothing else is.
+// rounded to the 16-bit type as operands of the next product (half a step each, averaged over the keys; fp16
+// turns a dS beyond 65504 into an infinity, as a loss scale that is too large does elsewhere), as are the outputs;
+// nothing else is.
 //
-//   cross_fwd_kernel   128 rows (4 waves x 32), key tiles of 64 double-buffered in LDS
+//   cross_fwd_kernel   128 rows (4 waves x 32), key tiles of 64 in LDS
 //   cross_few_kernel   up to 32 rows (single tokens): every wave goes through key tiles of its own, keys
 //                      straight into registers, values through a small LDS tile of the wave; joined in LDS
 //   cross_dq_kernel    128 rows over all key tiles; also D_r
@@ -20,7 +21,18 @@
 //
 // S is computed transposed (keys on the matrix rows, query rows on the lanes), so that a row's maximum and sum
 // are lane-local plus one exchange of the wave's halves, and the accumulators are the next product's operand
-// as they stand; V^T, K^T, Q^T and dO^T come from ds_read_b64_tr_b16 reads of row-major LDS tiles.
+// as they stand; V^T, K^T, Q^T and dO^T come from ds_read_b64_tr_b16 reads of row-major LDS tiles. Tiles come by
+// buffer loads that write LDS without passing registers, one or two tiles ahead of their use, one barrier a tile.
+//
+// What bounds it (MI355X, bf16; a large matrix product reaches 1367 TFLOP/s and a large copy 5.0 TB/s here):
+//   long rows      the matrix cores at the clock that the power allows (about 1.6 GHz then). 4 x 4096 x 4096, 16
+//                  heads of 128: forward 557 us (988 TFLOP/s), dQ 714 (1155), dK and dV 1046 (1051); all three
+//                  2121 us. Two kernels without atomics compute S and dP twice: 18 products' work for 14.
+//                  16 heads of 64: forward 335 us (821), dQ 405 (1018), dK and dV 609 (903): the exponentials and
+//                  sums of a tile take as long as its products.
+//   short rows     latency of a tile and of a launch: 8 x 512 x 512 ragged, 16 heads of 64: 18, 23 and 28 us
+//   single tokens  memory: 32 tokens over 1500 ragged states, 16 heads of 64: 39 us (3.8 TB/s); one token over
+//                  131071 states, 8 key heads of 128: 104 us with its join (5.2 TB/s)
 #include "fused_common.h"
 
 #include <algorithm>
@@ -461,7 +473,8 @@ __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
   }
 }
 
-// Up to 32 rows: wave w takes the 32-key tiles w, w + 4, ... of the split.
+// Up to 32 rows: wave w takes the 32-key tiles w, w + 4, ... of the split. Bound by memory: with the loads of two
+// tiles under way per wave (heads of 64), 32 tokens over 1500 states take 39 us, with one 45 us.
 template <typename E, int DP>
 __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   typedef Tile<DP> L;
@@ -793,7 +806,8 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   }
 }
 
-// 128 keys, key on the lane; row tiles of RT through LDS.
+// 128 keys, key on the lane; row tiles of RT through LDS. With wide heads K, dK and dV fill the registers, V comes from
+// LDS; two waves sharing 32 keys, each with half of the columns, leave room but wait more (1235 us for 1050).
 template <typename E, int DP, int RT>
 __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   typedef Tile<DP> L;
@@ -971,7 +985,7 @@ void split_axis(CrossParams& p, int64_t have, int len, int tile) {
 
 unsigned grid_of(const CrossParams& p) {
   const int64_t g = (int64_t)p.blocks * p.splits * p.B * p.N;
-  TORCH_CHECK(g < (1ll << 31), "cross_attention: too many workgroups");
+  TORCH_CHECK(g < (1ll << 24), "cross_attention: fewer than 2^24 workgroups wanted (sequences x key heads x blocks of 128)");
   return (unsigned)g;
 }
 
@@ -994,6 +1008,7 @@ CrossParams cross_params(const at::Tensor& q, const at::Tensor& kv, const OptTen
   p.kv = (const u16*)kv.data_ptr();
   p.qb = q.stride(0), p.qt = q.stride(1), p.qh = q.stride(2);
   p.kb = kv.stride(0), p.kt = kv.stride(1), p.ks = kv.stride(2), p.kh = kv.stride(3);
+  if (kv.size(1) == 1) p.kt = 2 * kv.size(3) * kv.size(4);  // a single state may have any stride; rows behind it are outside
   p.B = (int)q.size(0), p.Tq = (int)q.size(1), p.Tk = (int)kv.size(1), p.N = (int)kv.size(3), p.D = (int)q.size(3);
   p.G = (int)(q.size(2) / kv.size(3));
   p.M = p.G * p.Tq;
@@ -1153,6 +1168,7 @@ at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& kv, const OptT
   TORCH_CHECK(kv.size(3) > 0 && q.size(2) > 0 && q.size(2) % kv.size(3) == 0, op, "N must divide H");
   TORCH_CHECK(q.size(1) * q.size(2) < (1ll << 31) - kRows && kv.size(1) < (1ll << 31) - kRows && q.size(0) < (1ll << 31), op,
               "fewer than 2^31 rows and states wanted");
+  TORCH_CHECK(q.size(2) * q.size(3) <= (1 << 20), op, "H times D of at most 2^20 wanted");  // a tile's offsets fit 31 bits
   TORCH_CHECK(std::isfinite(scale) && scale > 0.0, op, "scale must be positive");
   OptTensor len;
   if (lengths) {

@@ -288,6 +288,11 @@ def test_empty_and_refusals_gpu():
                  lambda: fused.cross_attention(torch.cat([q] * 3, -1), torch.cat([kv] * 3, -1))):
         with pytest.raises(RuntimeError, match="multiple of 8 up to 128"):
             call()
+    many = torch.zeros(1 << 24, 1, 1, 8, device=dev, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="workgroups"):
+        fused.cross_attention(many, many[:, :, None].expand(-1, -1, 2, -1, -1))
+    with pytest.raises(RuntimeError, match="2\\^20"):
+        fused.cross_attention(torch.zeros(1, 1, 1 << 15, 64, device=dev).half(), torch.zeros(1, 1, 2, 1, 64, device=dev).half())
     with pytest.raises(ValueError, match="lengths"):
         fused.cross_attention(q, kv, torch.tensor([3]))
     with pytest.raises(RuntimeError, match="second derivatives"):

@@ -295,3 +295,19 @@ def test_more_than_two_to_the_31_elements():
         assert torch.equal(y[row].cpu(), want), row
     share = (y != 0).sum(dtype=torch.int64).item() / y.numel()
     assert abs(share - 0.5) < 5 * 0.5 / math.sqrt(y.numel())
+
+
+@gpu
+def test_norm_of_more_rows_than_one_launch_takes():
+    """Rows beyond 2^22 blocks of four: x = 0 and delta = 1, so that s is the mask and y follows from its count."""
+    dev = _cuda()
+    rows, d = (1 << 24) + 6, 136
+    s, y = fused.dropout_add_rms_norm(torch.zeros(rows, d, device=dev, dtype=torch.bfloat16),
+                                      torch.ones(rows, d, device=dev, dtype=torch.bfloat16),
+                                      torch.ones(d, device=dev, dtype=torch.bfloat16), 0.5, SEED, eps=0.0)
+    for row in (0, (1 << 24) - 1, 1 << 24, rows - 1):
+        words = [_philox([c // 4, row, 0, 0], [SEED & 0xFFFFFFFF, SEED >> 32])[c % 4] for c in range(d)]
+        want = torch.tensor([2.0 if v >= 1 << 31 else 0.0 for v in words], dtype=torch.float64)
+        assert torch.equal(s[row].double().cpu(), want), row
+        ref = want * want.square().mean().rsqrt()
+        assert ((y[row].double().cpu() - ref).abs() <= 1.01 * 2.0 ** -8 * ref).all(), row

@@ -36,6 +36,7 @@
 #include "fused_common.h"
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -198,6 +199,15 @@ __device__ __forceinline__ unsigned bytes_of(int valid, int64_t stride, int D) {
   return valid <= 0 ? 0u : (unsigned)min(((int64_t)(valid - 1) * stride + D) * 2, (int64_t)kOutside - 1);
 }
 
+// The builtin is younger than the instruction: a compiler without it (a pod's image may have one) gets the intrinsic
+// by its name, the same code.
+#if defined(__HIP_DEVICE_COMPILE__) && !__has_builtin(__builtin_amdgcn_raw_ptr_buffer_load_lds)
+extern "C" __device__ void buffer_load_to_lds(__amdgpu_buffer_rsrc_t src, lds_void* lds, int size, int offset, int soffset,
+                                              int at, int aux) __asm("llvm.amdgcn.raw.ptr.buffer.load.lds");
+#else
+#define buffer_load_to_lds __builtin_amdgcn_raw_ptr_buffer_load_lds
+#endif
+
 // BYTES (4 or 16) per lane from `base` plus this lane's offset to `lds` plus BYTES times the lane, without passing
 // registers
 template <int BYTES>
@@ -205,8 +215,8 @@ __device__ __forceinline__ void to_lds(const void* base, unsigned bytes, void* l
   static_assert(BYTES == 16 || BYTES == 4, "sizes used here");
 #ifdef __HIP_DEVICE_COMPILE__  // the buffer's type is the device's
   __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
-  if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(lds_u8*)lds, 16, offset, 0, 0, 0);
-  else __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(lds_u8*)lds, 4, offset, 0, 0, 0);
+  if constexpr (BYTES == 16) buffer_load_to_lds(src, (lds_void*)(lds_u8*)lds, 16, offset, 0, 0, 0);
+  else buffer_load_to_lds(src, (lds_void*)(lds_u8*)lds, 4, offset, 0, 0, 0);
 #endif
 }
 

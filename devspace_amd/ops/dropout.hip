@@ -21,6 +21,7 @@
 #include "fused_common.h"
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 namespace {

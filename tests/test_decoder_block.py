@@ -102,3 +102,41 @@ def test_one_token_is_a_row_of_the_sequence():
             # two kernels with the same roundings in another order: probabilities 2^-8 each, the outputs too
             size = kv[:, :, 1].float().abs().amax()
             assert ((one - o[:, t:t + 1]).abs() <= 4 * 2.0 ** -8 * size).all()
+
+
+@gpu
+def test_two_streams_at_once():
+    """The same calls on two streams, none waiting for another, against the same calls alone: workspaces are the
+    call's own. Long enough on the device that they overlap."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    fused.ext()
+    torch.manual_seed(3)
+    dev = "cuda"
+    freqs = fused.rotary_frequencies(D, device=dev)[0]
+    sets = []
+    for i in range(2):
+        q = torch.randn(1, 600, 2, D, device=dev).bfloat16().requires_grad_()
+        kv = torch.randn(1, 3000, 2, 2, D, device=dev).bfloat16().requires_grad_()  # both axes split
+        w = torch.ones(D, device=dev).bfloat16().requires_grad_()
+        sets.append((q, kv, w, torch.randn_like(q)))
+
+    def run(s, seed):
+        q, kv, w, g = s
+        t = fused.rotary(q, seed, freqs)
+        o = fused.cross_attention(t, kv)
+        _, y = fused.dropout_add_rms_norm(t, o, w, 0.2, seed)
+        return [y.detach(), *torch.autograd.grad(y, (q, kv, w), g)]
+
+    want = [run(s, 5 + i) for i, s in enumerate(sets)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for i, (s, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got.append(run(s, 5 + i))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)

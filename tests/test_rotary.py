@@ -257,12 +257,23 @@ def test_captured_and_replayed_on_another_stream():
     with torch.cuda.stream(side):
         fused.rotary_qk(q, k, pos, f)
     torch.cuda.current_stream().wait_stream(side)
+    leaf = torch.randn(2, 9, 3, 4, 64, device=dev).half().requires_grad_()
+    start, grad = torch.zeros(9, dtype=torch.int32, device=dev), torch.randn(2, 9, 3, 4, 64, device=dev).half()
+
+    def train():
+        y = fused.rotary_qkv(leaf, start, f, interleaved=True)
+        return [y.detach(), *torch.autograd.grad(y, leaf, grad)]
+
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         yq, yk = fused.rotary_qk(q, k, pos, f)
+        trained = train()
     for step in range(4):
         pos += 1000 * step + 1
+        start += 7
         g.replay()
         torch.cuda.synchronize()
         eq, ek = fused.rotary_qk(q, k, pos, f)
         assert torch.equal(yq, eq) and torch.equal(yk, ek)
+        for a, b in zip(trained, train()):
+            assert torch.equal(a, b)

@@ -316,6 +316,28 @@ def test_far_offsets():
 
 
 @gpu
+def test_far_offsets_trained():
+    """The same for tiles of rows and their gradients: 2.25 * 2^30 elements of states in one sequence."""
+    dev = _cuda()
+    tk, heads, d, tq = 1_100_003, 8, 128, 40
+    q = torch.randn(1, 1, heads, d, device=dev).bfloat16().expand(1, tq, heads, d).contiguous().requires_grad_()
+    kv = torch.zeros(1, tk, 2, heads, d, device=dev, dtype=torch.bfloat16)
+    kv[:, -1, 0] = 40 * q[:, 0].detach()
+    kv[:, -1, 1] = torch.randn(1, heads, d, device=dev).bfloat16()
+    kv.requires_grad_()
+    do = torch.randn(1, tq, heads, d, device=dev).bfloat16()
+    o = fused.cross_attention(q, kv)
+    assert torch.equal(o, kv[:, -1:, 1].expand_as(o))
+    dq, dkv = torch.autograd.grad(o, (q, kv), do)
+    want = do.double().sum(1)  # P = 1 for the last state: 40 terms summed in 32 bits, rounded once
+    off = (dkv[:, -1, 1].double() - want).abs()
+    assert (off <= 2.0 ** -8 * want.abs() + 40 * U * do.double().abs().sum(1)).all()
+    assert not dkv[:, :-1].any()
+    # dS = dP - dO . O: both sums of 128 products in 32 bits; times K of up to 40 * 5 and its scale
+    assert dq.abs().max() <= 256 * U * 128 * 25 * 200
+
+
+@gpu
 def test_captured_with_lengths_read_at_each_replay():
     dev = _cuda()
     q, kv, do = _inputs(dev, torch.bfloat16, 2, 40, 600, 4, 2, 64)

@@ -775,7 +775,9 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
       for (int nb = 0; nb < L::NB; ++nb) dq[nb] = mfma<E>(lds.tr8(Ks, kb * 32 + 16 * ks, nb), db, dq[nb]);
     }
   };
-  if (p.splits == 1 && k_end <= kKeys) {
+  if (p.splits == 1 && k_end <= 1) {
+    // the softmax of a single state is constant: dQ = 0, and nothing of P's last bits in it
+  } else if (p.splits == 1 && k_end <= kKeys) {
     // One tile holds all states. With few of them, the rounding of O weighs in dO . O, which nearly equals the
     // dP it is taken from; here it is summed from P and dP themselves.
     key_loop<DP>(tile0, tile1, tile2, p, w, wave, lane, k_begin, k_end, [&](const unsigned char* Ks, const unsigned char* Vs, int k0) {
@@ -913,6 +915,10 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (r0 + qs * 32 + acc_row(i, hh) >= r_end) s[i] = dp[i] = 0.f;
+      }
+      if (len == 1) {  // a single state: dK = 0
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] = 0.f;
       }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {

@@ -7,7 +7,8 @@
 //   dropout_add           s = x + dropout(delta)
 //   dropout_add_rms_norm  s as above, y = s r w, r = rsqrt(mean s^2 + eps)
 //   backward of the last  g = ds + r w dy - s r^3 / D sum(w dy s), dx = g, ddelta = dropout(g),
-//                         dw = sum over rows of dy s r
+//                         dw = sum over rows of dy s r, with s summed again from x and delta: the rounded
+//                         s would weigh in dw (up to 1.75 times the rounding of dw itself)
 //
 // Philox 4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3",
 // 2011): the backward pass computes the same words again instead of reading a mask. A block of four words
@@ -64,17 +65,24 @@ __device__ __forceinline__ void philox(unsigned c0, unsigned c1, unsigned c2, un
   w[0] = c0, w[1] = c1, w[2] = c2, w[3] = c3;
 }
 
-// The eight elements at column 8 v of a row, kept and scaled or dropped. What is dropped becomes 0
-// whatever it was (a product with the mask would make NaN of an infinity).
-__device__ __forceinline__ void drop8(float f[8], int64_t row, unsigned v, const Key& k) {
+// Which of the eight elements at column 8 v of a row stay, a bit each.
+__device__ __forceinline__ unsigned keep8(int64_t row, unsigned v, const Key& k) {
+  unsigned bits = 0;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     unsigned w[4];
     philox(2 * v + q, (unsigned)row, (unsigned)((uint64_t)row >> 32), k.offset, k.k0, k.k1, w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[4 * q + i] = (w[i] > k.last || k.none) ? f[4 * q + i] * k.scale : 0.f;
+    for (int i = 0; i < 4; ++i) bits |= (w[i] > k.last || k.none) ? 1u << (4 * q + i) : 0u;
   }
+  return bits;
 }
+// They are scaled; what is dropped becomes 0 whatever it was (a product with the mask would make NaN of an infinity).
+__device__ __forceinline__ void drop8(float f[8], unsigned bits, float scale) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = bits >> i & 1 ? f[i] * scale : 0.f;
+}
+__device__ __forceinline__ void drop8(float f[8], int64_t row, unsigned v, const Key& k) { drop8(f, keep8(row, v, k), k.scale); }
 
 // Up to eight elements of a row as they are stored, 0 behind its end: one wide access, or the row's last n in pieces
 // of four, two and one. EVEN: rows are whole groups of eight. They are widened where they are used, so that no load
@@ -154,37 +162,45 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const typename E::S* 
 
 // ------------------------------------------------------------------------------ dropout + add + norm
 
-// Sum over the lanes that share a row: part of a wave, a wave, or the block's four waves through LDS.
+// threads of a block that gives each row LANES lanes
+constexpr int threads_for(int lanes) { return lanes < kThreads ? kThreads : lanes; }
+
+// Sum over the lanes that share a row: part of a wave, a wave, or the block's waves through LDS, in their order.
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
   for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  if (LANES <= 64) return v;
-  const int wave = threadIdx.x >> 6;
-  __syncthreads();  // the last row's sums have been read
-  if ((threadIdx.x & 63) == 0) red[wave] = v;
-  __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  if constexpr (LANES <= 64) {
+    return v;
+  } else {
+    __syncthreads();  // the last row's sums have been read
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < LANES / 64; ++i) t += red[i];
+    return t;
+  }
 }
 
-// LANES lanes per row (4 to 64, or the block's 256), VPL groups of eight elements per lane: lane l owns groups l, l + LANES, ...
+// LANES lanes per row (4 to 64, or the block's 256 to 1024), VPL groups of eight elements per lane: lane l owns groups l, l + LANES, ...
 // and keeps them in registers between the sum of squares and the scaled store, so that each tensor passes once.
 template <typename E, int LANES, int VPL, bool EVEN>
-__global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename E::S* __restrict__ x,
+__global__ void __launch_bounds__(threads_for(LANES)) drop_norm_fwd_kernel(const typename E::S* __restrict__ x,
                                                                  const typename E::S* __restrict__ delta,
                                                                  const typename E::S* __restrict__ w,
                                                                  typename E::S* __restrict__ sum,
                                                                  typename E::S* __restrict__ y, float* __restrict__ rstd,
                                                                  int64_t row0, int64_t R, int D, float eps, Drop drop) {
-  __shared__ float red[4];
+  __shared__ float red[16];
+  constexpr int kRows = threads_for(LANES) / LANES;  // of a block
   const int lane = threadIdx.x & (LANES - 1);
-  const int64_t row = row0 + (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  if (LANES < kThreads && row >= R) return;
+  const int64_t row = row0 + (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
+  if (kRows > 1 && row >= R) return;
   const Key key(drop);
   const int nvec = (D + 7) >> 3;
   const int64_t base = row * D;
-  // the weight is loaded with the row, not behind its sum, where the registers hold it
-  constexpr bool kEarly = VPL <= 4;
+  // the weight is loaded with the row, not behind its sum
   Pack<typename E::S, 8> rx[VPL], rd[VPL], rw[VPL];
   float s[VPL][8];
 #pragma unroll
@@ -193,7 +209,7 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
     if (i < nvec) {
       rx[k] = load8<typename E::S, EVEN>(x + base + 8 * i, D - 8 * i);
       rd[k] = load8<typename E::S, EVEN>(delta + base + 8 * i, D - 8 * i);
-      if (kEarly) rw[k] = load8<typename E::S, EVEN>(w + 8 * i, D - 8 * i);
+      rw[k] = load8<typename E::S, EVEN>(w + 8 * i, D - 8 * i);
     }
   }
   float ss = 0.f;
@@ -221,7 +237,6 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
     const int i = lane + LANES * k;
     if (i < nvec) {
       float wv[8];
-      if (!kEarly) rw[k] = load8<typename E::S, EVEN>(w + 8 * i, D - 8 * i);
       widen<E>(rw[k], wv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[k][j] *= r * wv[j];
@@ -234,13 +249,13 @@ __global__ void __launch_bounds__(kThreads) drop_norm_fwd_kernel(const typename 
 // its columns in registers, and the block writes one fp32 row of partial sums, which part_sum_kernel adds in a
 // fixed order.
 template <typename E, int LANES, int VPL, bool EVEN>
-__global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
-    const typename E::S* __restrict__ dy, const typename E::S* __restrict__ ds, const typename E::S* __restrict__ s,
-    const typename E::S* __restrict__ w, const float* __restrict__ rstd, typename E::S* __restrict__ dx,
+__global__ void __launch_bounds__(threads_for(LANES)) drop_norm_bwd_kernel(
+    const typename E::S* __restrict__ dy, const typename E::S* __restrict__ ds, const typename E::S* __restrict__ x,
+    const typename E::S* __restrict__ delta, const typename E::S* __restrict__ w, const float* __restrict__ rstd, typename E::S* __restrict__ dx,
     typename E::S* __restrict__ dd, float* __restrict__ part, int64_t R, int D, int rows_per_block, Drop drop) {
-  __shared__ float red[4];
-  constexpr int kStep = kThreads / LANES;  // groups
-  extern __shared__ float sdw[];           // [kStep][D], with more than one
+  __shared__ float red[16];
+  constexpr int kStep = threads_for(LANES) / LANES;  // groups
+  extern __shared__ float sdw[];                     // [kStep][D], with more than one
   const int lane = threadIdx.x & (LANES - 1);
   const Key key(drop);
   const int nvec = (D + 7) >> 3;
@@ -251,19 +266,16 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
     for (int j = 0; j < 8; ++j) acc[k][j] = 0.f;
   const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = min(R, r0 + rows_per_block);
   const float inv_d = 1.0f / (float)D;
-  // kept in registers where they fit beside the weight gradient: the weight over all rows, and the residual's
-  // gradient from the row's first loads on
-  constexpr bool kKeepW = VPL <= 2, kEarly = VPL <= 4;
   typedef Pack<typename E::S, 8> Raw;
-  Raw rw[VPL], rr[VPL], rg[VPL], rs[VPL];
-  if (kKeepW) {
+  Raw rw[VPL], rr[VPL], rg[VPL], rx[VPL], rd[VPL];
 #pragma unroll
-    for (int k = 0; k < VPL; ++k)
-      if (lane + LANES * k < nvec) rw[k] = load8<typename E::S, EVEN>(w + 8 * (lane + LANES * k), D - 8 * (lane + LANES * k));
+  for (int k = 0; k < VPL; ++k) {
+    if (lane + LANES * k < nvec) rw[k] = load8<typename E::S, EVEN>(w + 8 * (lane + LANES * k), D - 8 * (lane + LANES * k));
   }
   for (int64_t row = r0 + threadIdx.x / LANES; row < r1; row += kStep) {
     const int64_t base = row * D;
     float g[VPL][8], sv[VPL][8];
+    unsigned keep[VPL];
     float dot = 0.f;
     const float r = rstd[row];
 #pragma unroll
@@ -271,20 +283,24 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
       const int i = lane + LANES * k, n = D - 8 * i;
       if (i < nvec) {
         if (dy) rg[k] = load8<typename E::S, EVEN>(dy + base + 8 * i, n);
-        rs[k] = load8<typename E::S, EVEN>(s + base + 8 * i, n);
-        if (kEarly && ds) rr[k] = load8<typename E::S, EVEN>(ds + base + 8 * i, n);
-        if (!kKeepW) rw[k] = load8<typename E::S, EVEN>(w + 8 * i, n);
+        rx[k] = load8<typename E::S, EVEN>(x + base + 8 * i, n);
+        rd[k] = load8<typename E::S, EVEN>(delta + base + 8 * i, n);
+        if (ds) rr[k] = load8<typename E::S, EVEN>(ds + base + 8 * i, n);
       }
     }
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
       if (lane + LANES * k < nvec) {
-        float wv[8];
+        float wv[8], d[8];
+        keep[k] = keep8(row, lane + LANES * k, key);
         widen<E>(rg[k], g[k]);
-        widen<E>(rs[k], sv[k]);
+        widen<E>(rx[k], sv[k]);
+        widen<E>(rd[k], d);
         widen<E>(rw[k], wv);
+        drop8(d, keep[k], key.scale);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          sv[k][j] += d[j];
           if (!dy) g[k][j] = 0.f;
           acc[k][j] += g[k][j] * sv[k][j] * r;
           g[k][j] *= wv[j];
@@ -299,18 +315,17 @@ __global__ void __launch_bounds__(kThreads) drop_norm_bwd_kernel(
       const int i = lane + LANES * k, n = D - 8 * i;
       if (i < nvec) {
         float rv[8];
-        if (!kEarly && ds) rr[k] = load8<typename E::S, EVEN>(ds + base + 8 * i, n);
         widen<E>(rr[k], rv);
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[k][j] = r * g[k][j] - sv[k][j] * c + (ds ? rv[j] : 0.f);
         store8<E, EVEN>(dx + base + 8 * i, n, g[k]);
-        drop8(g[k], row, i, key);
+        drop8(g[k], keep[k], key.scale);
         store8<E, EVEN>(dd + base + 8 * i, n, g[k]);
       }
     }
   }
   float* out = part + (int64_t)blockIdx.x * D;
-  if (LANES < kThreads) {
+  if constexpr (kStep > 1) {
     float* mine = sdw + threadIdx.x / LANES * D;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
@@ -427,24 +442,25 @@ at::Tensor dropout_apply(const at::Tensor& d, const at::Tensor& x, const Drop& d
 }
 
 // Lanes per row and groups per lane of the norm kernels: as many lanes as a narrow row has groups (several rows
-// per wave: 4128008 rows x 22 forward and backward take 1 wave per row 8709 us), a wave per row up to 2048 columns
-// (no barrier, four rows in flight per block), the whole block beyond.
+// per wave: 4128008 rows x 22 forward and backward take 1 wave per row 8709 us, so 619), a wave per row up to 1024
+// columns (no barrier, four rows in flight per block), a block per row beyond, never more than two groups a lane.
 template <typename F>
 void by_width(int64_t D, F&& g) {
-  using std::integral_constant;
   auto f = [&](auto lanes, auto vpl) {
     if (D % 8 == 0) g(lanes, vpl, std::true_type{});
     else g(lanes, vpl, std::false_type{});
   };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
   const int64_t n = (D + 7) / 8;
-  if (n <= 4) f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  else if (n <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-  else if (n <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  else if (n <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  else if (n <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  else if (n <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  else if (n <= 1024) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  else f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+  if (n <= 4) f(std::integral_constant<int, 4>{}, one);
+  else if (n <= 16) f(std::integral_constant<int, 16>{}, one);
+  else if (n <= 64) f(std::integral_constant<int, 64>{}, one);
+  else if (n <= 128) f(std::integral_constant<int, 64>{}, two);
+  else if (n <= 256) f(std::integral_constant<int, 256>{}, one);
+  else if (n <= 512) f(std::integral_constant<int, 256>{}, two);
+  else if (n <= 1024) f(std::integral_constant<int, 512>{}, two);
+  else f(std::integral_constant<int, 1024>{}, two);
 }
 
 struct NormForward {
@@ -460,10 +476,10 @@ NormForward drop_norm_fwd(const at::Tensor& x, const at::Tensor& delta, const at
     typedef decltype(e) E;
     typedef typename E::S S;
     by_width(D, [&](auto lanes, auto vpl, auto even) {
-      const int64_t at_once = kThreads / lanes, most = at_once << 22;  // rows of one launch
+      const int64_t at_once = threads_for(lanes) / lanes, most = at_once << 21;  // rows of one launch
       for (int64_t row0 = 0; row0 < R; row0 += most) {
         const int64_t blocks = (std::min(most, R - row0) + at_once - 1) / at_once;
-        hipLaunchKernelGGL((drop_norm_fwd_kernel<E, lanes, vpl, even>), dim3((unsigned)blocks), dim3(kThreads), 0, stream(),
+        hipLaunchKernelGGL((drop_norm_fwd_kernel<E, lanes, vpl, even>), dim3((unsigned)blocks), dim3(threads_for(lanes)), 0, stream(),
                            (const S*)x.data_ptr(), (const S*)delta.data_ptr(), (const S*)w.data_ptr(), (S*)o.sum.data_ptr(),
                            (S*)o.y.data_ptr(), o.rstd.data_ptr<float>(), row0, R, (int)D, (float)eps, drop);
         LAUNCH_CHECK();
@@ -474,25 +490,26 @@ NormForward drop_norm_fwd(const at::Tensor& x, const at::Tensor& delta, const at
 }
 
 // dy or ds may be undefined (zero)
-std::vector<at::Tensor> drop_norm_bwd(const at::Tensor& dy, const at::Tensor& ds, const at::Tensor& s, const at::Tensor& w,
-                                      const at::Tensor& rstd, const Drop& drop) {
-  c10::DeviceGuard guard(s.device());
-  const int64_t D = s.size(-1), R = D ? s.numel() / D : 0;
-  auto dx = at::empty_like(s), dd = at::empty_like(s), dw = at::empty_like(w);
+std::vector<at::Tensor> drop_norm_bwd(const at::Tensor& dy, const at::Tensor& ds, const at::Tensor& x, const at::Tensor& delta,
+                                      const at::Tensor& w, const at::Tensor& rstd, const Drop& drop) {
+  c10::DeviceGuard guard(x.device());
+  const int64_t D = x.size(-1), R = D ? x.numel() / D : 0;
+  auto dx = at::empty_like(x), dd = at::empty_like(x), dw = at::empty_like(w);
   if (R == 0) return {dx, dd, dw.zero_()};
-  by_type(s.scalar_type(), [&](auto e) {
+  by_type(x.scalar_type(), [&](auto e) {
     typedef decltype(e) E;
     typedef typename E::S S;
     by_width(D, [&](auto lanes, auto vpl, auto even) {
       // two rows per group of lanes; at most 1024 rows of partial sums
-      const int64_t at_once = kThreads / lanes;
+      const int64_t at_once = threads_for(lanes) / lanes;
       const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(1024, (R + 2 * at_once - 1) / (2 * at_once)));
       const int64_t per = (R + blocks - 1) / blocks;
       TORCH_CHECK(per < (1ll << 31), "dropout_add_rms_norm: too many rows");
-      auto part = at::empty({blocks, D}, s.options().dtype(at::kFloat));
-      hipLaunchKernelGGL((drop_norm_bwd_kernel<E, lanes, vpl, even>), dim3((unsigned)blocks), dim3(kThreads),
+      auto part = at::empty({blocks, D}, x.options().dtype(at::kFloat));
+      hipLaunchKernelGGL((drop_norm_bwd_kernel<E, lanes, vpl, even>), dim3((unsigned)blocks), dim3(threads_for(lanes)),
                          at_once > 1 ? at_once * D * sizeof(float) : 0, stream(), dy.defined() ? (const S*)dy.data_ptr() : nullptr,
-                         ds.defined() ? (const S*)ds.data_ptr() : nullptr, (const S*)s.data_ptr(), (const S*)w.data_ptr(),
+                         ds.defined() ? (const S*)ds.data_ptr() : nullptr, (const S*)x.data_ptr(),
+                         (const S*)delta.data_ptr(), (const S*)w.data_ptr(),
                          rstd.data_ptr<float>(), (S*)dx.data_ptr(), (S*)dd.data_ptr(), part.data_ptr<float>(), R, (int)D,
                          (int)per, drop);
       LAUNCH_CHECK();
@@ -544,9 +561,9 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
 struct DropNormFn : public torch::autograd::Function<DropNormFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& delta, const at::Tensor& w,
                                double eps, double p, int64_t seed, const OptTensor& seed_at, int64_t offset) {
-    auto wc = w.contiguous();
-    auto o = drop_norm_fwd(x.contiguous(), delta.contiguous(), wc, eps, make_drop(p, seed, seed_at, offset));
-    ctx->save_for_backward({o.sum, wc, o.rstd, seed_at ? *seed_at : at::Tensor()});
+    auto xc = x.contiguous(), dc = delta.contiguous(), wc = w.contiguous();
+    auto o = drop_norm_fwd(xc, dc, wc, eps, make_drop(p, seed, seed_at, offset));
+    ctx->save_for_backward({xc, dc, wc, o.rstd, seed_at ? *seed_at : at::Tensor()});
     save_drop(ctx, p, seed, offset);
     ctx->set_materialize_grads(false);
     return {o.sum, o.y};
@@ -557,7 +574,7 @@ struct DropNormFn : public torch::autograd::Function<DropNormFn> {
     auto dense = [](const at::Tensor& g) { return g.defined() ? g.contiguous() : g; };
     at::Tensor none;
     if (!grads[0].defined() && !grads[1].defined()) return {none, none, none, none, none, none, none, none};
-    auto r = drop_norm_bwd(dense(grads[1]), dense(grads[0]), s[0], s[1], s[2], saved_drop(ctx, s[3]));
+    auto r = drop_norm_bwd(dense(grads[1]), dense(grads[0]), s[0], s[1], s[2], s[3], saved_drop(ctx, s[4]));
     return {r[0], r[1], r[2], none, none, none, none, none};
   }
 };

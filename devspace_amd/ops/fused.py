@@ -1,4 +1,4 @@
-"""Autograd wrappers around the gfx950 fused ops (fused_ops.hip).
+"""Autograd wrappers around the gfx950 fused ops (fused_ops.hip, rotary.hip, dropout.hip, cross_attention.hip).
 
     from devspace_amd.ops import fused
     norm = fused.RMSNorm(dim)             # drop-in for nn.RMSNorm
@@ -62,8 +62,8 @@ def ext():
 
 
 def _check_source(mod) -> None:
-    """An in-tree build must come from the source next to it: kernels older than an edit of
-    fused_ops.hip must not run (an error, not a silent fallback)."""
+    """An in-tree build must come from the sources next to it: kernels older than an edit of
+    them must not run (an error, not a silent fallback)."""
     import os
 
     from . import build
@@ -76,8 +76,8 @@ def _check_source(mod) -> None:
 
 
 def check_fresh() -> str:
-    """The loaded extension was built from the fused_ops.hip next to it: returns the source
-    SHA-256, raises on a stale build (kernels older than the source)."""
+    """The loaded extension was built from the sources next to it: returns their SHA-256, raises
+    on a stale build (kernels older than the sources)."""
     from . import build
 
     _check_source(ext())
@@ -438,8 +438,9 @@ def dropout_add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Ten
                          eps: float | None = None, offset: int = 0):
     """add_rms_norm() of a residual stream with dropout: returns (s, y) with
     s = x + dropout(delta, p, seed, offset) and y = rms_norm(s) * weight, one kernel each way (and a
-    small one for the weight's gradient). y is made of the sum before it is rounded to s. On a GPU rows
-    (the last dimension) of up to 16384 elements."""
+    small one for the weight's gradient). y and the gradients are made of the sum before it is rounded
+    to s: the backward pass sums x and delta again. On a GPU rows (the last dimension) of up to 16384
+    elements."""
     seed, at = _check_dropout("dropout_add_rms_norm", p, seed, offset, x.dtype)
     if x.shape != delta.shape or x.dtype != delta.dtype or x.device != delta.device:
         raise ValueError("dropout_add_rms_norm: x and delta must agree in shape, type and device")

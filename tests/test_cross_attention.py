@@ -167,6 +167,21 @@ def test_forward_and_backward(dtype, b, tq, tk, h, g, d, lengths):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,tq,g,d", [("bf16", 1, 1, 64), ("fp16", 70, 2, 128), ("bf16", 40, 4, 80)])
+def test_a_single_state(dtype, tq, g, d):
+    """Its softmax is constant: O = V to the bit, dQ = dK = 0 exactly."""
+    dev = _cuda()
+    q, kv, do = _inputs(dev, DTYPES[dtype], 2, tq, 5, 4, g, d, big=3.0)
+    n = torch.tensor([1, 0], device=dev)
+    for x, lengths in ((kv, n), (kv[:, :1], None)):
+        x = x.detach().clone().requires_grad_()
+        got = _run(q, x, do, lengths)
+        _hold(got, q, x, do, lengths)
+        assert not got["dq"].any() and not got["dkv"][:, :, 0].any()
+        assert torch.equal(got["o"][0], x[0, :1, 1].repeat_interleave(g, 1).expand(tq, -1, -1))
+
+
+@gpu
 def test_frozen_states_and_frozen_queries():
     dev = _cuda()
     q, kv, do = _inputs(dev, torch.bfloat16, 2, 50, 1000, 4, 2, 64)

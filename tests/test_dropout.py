@@ -178,19 +178,14 @@ def test_dropout_add_rms_norm_forward_and_backward(dtype, rows, dim, use):
     u = cy * f64(w)
     dot = (u * t).sum(-1, keepdim=True)
     g = cs + r * u - t * r ** 3 * dot / dim
-    # the backward pass reads the rounded sum: each of its elements off by half a step of the type. In g that
-    # is half a step of the dot's terms (independent, six standard deviations of their sum, and never more than
-    # their sizes added) and of t itself, and the 32-bit steps
-    h = _half_step(dt)
-    noise = torch.minimum((u * t).abs().sum(-1, keepdim=True), 6 * (u * t).square().sum(-1, keepdim=True).sqrt())
-    size = (u * t).abs().sum(-1, keepdim=True)
-    before = t.abs() * r ** 3 / dim * (h * noise + h * dot.abs() + 4 * steps * U * size) + \
+    # the backward pass in 32 bits: the sum is off by 3 u of its parts, its row's sum by `steps` u of its terms' sizes
+    size = (u * t).abs().sum(-1, keepdim=True) + (u.abs() * part / U).sum(-1, keepdim=True)
+    before = t.abs() * r ** 3 / dim * 4 * steps * U * size + part * r ** 3 / dim * dot.abs() + \
         4 * steps * U * (cs.abs() + (r * u).abs())
     _close(gx, g, before)
     _close(gd, g * factor, before * factor + 2 * U * (g * factor).abs())
-    terms = (cy * t * r).abs()
-    noise = torch.minimum(terms.sum(0), 6 * terms.square().sum(0).sqrt())
-    _close(gw, (cy * t * r).sum(0), h * noise + (steps + rows / 8 + 40) * U * terms.sum(0), extra=1e-30)
+    terms = (cy * r).abs() * (t.abs() + part / U)
+    _close(gw, (cy * t * r).sum(0), (steps + rows / 8 + 40) * U * terms.sum(0), extra=1e-30)
 
 
 @gpu

@@ -7,9 +7,8 @@
 // There is no causal mask, so the G query heads that share a key head are stacked: row m = t G + g, M = G Tq
 // rows over one set of keys, each key and value read once for all of them. All products run on
 // v_mfma_f32_32x32x16 (bf16 or fp16 in, fp32 out); softmax statistics and sums are in fp32. P and dS are
-// rounded to the 16-bit type as operands of the next product (half a step each, averaged over the keys; fp16
-// turns a dS beyond 65504 into an infinity, as a loss scale that is too large does elsewhere), as are the outputs;
-// nothing else is.
+// rounded to the 16-bit type as operands of the next product (half a step each, averaged over the keys; in fp16
+// by powers of two that keep them in its range), as are the outputs; nothing else is.
 //
 //   cross_fwd_kernel   128 rows (4 waves x 32), key tiles of 64 in LDS
 //   cross_few_kernel   up to 32 rows (single tokens): every wave goes through key tiles of its own, keys
@@ -109,6 +108,17 @@ struct Places {
     return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
+
+// Probabilities become operands of the 16-bit type. fp16 loses bits below 2^-14, and a probability of a long source is
+// smaller than that: they are lifted by a power of two, which what they are divided by, or the result, takes off
+// again (the sum l in the forward pass, whose P lies within 2^8 of its reference; 2^-kLiftBack in the backward pass,
+// whose P is at most 1). 65451 states in fp16: dK and dV were 2.2 times as far off as their own rounding.
+template <typename E>
+constexpr float kLift = E::kType == at::kHalf ? 7.f : 0.f;
+template <typename E>
+constexpr float kLiftBack = E::kType == at::kHalf ? 15.f : 0.f;
+template <typename E>
+constexpr float kUnliftBack = E::kType == at::kHalf ? 1.f / 32768.f : 1.f;
 
 // 2^x on the transcendental unit; 2^-inf = 0, which masked scores rely on
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -301,11 +311,42 @@ __device__ __forceinline__ float half_sum(float x) {
   return a + b;
 }
 
+// dS as an operand: fp16 neither holds the small values of long sources nor every large one, so each lane's column is
+// multiplied by a power of two that fits the largest value met so far (2^9 times the lift at the most). The
+// accumulators it goes into are rescaled when that falls; bf16 has the range and passes by.
+template <typename E>
+struct Gain {
+  float up = E::kType == at::kHalf ? 512.f : 1.f;
+  template <int NB>
+  __device__ __forceinline__ void fit(f32x16& ds, f32x16 (&acc)[NB]) {
+    if constexpr (E::kType == at::kHalf) {
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(ds[i]));
+      most = half_max(most);
+      if (__any(most * up > 32768.f)) {
+        const float fits = most > 0.f ? ldexpf(1.f, 15 - __builtin_amdgcn_frexp_expf(most)) : up;
+        const float next = fminf(up, fits), by = next / up;  // powers of two
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[nb][i] *= by;
+        up = next;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i] *= up;
+    }
+  }
+  // what the accumulators are multiplied by to be sums of dS
+  __device__ __forceinline__ float down() const { return kUnliftBack<E> / up; }
+};
+
 // One tile of scores in the log2 domain: the online softmax of this lane's row. On return s holds P against the
-// reference m, which follows the running maximum only when that has left it by more than 2^8: P and the sums stay
-// within 2^8 times the number of keys, nothing is lost in their floating types, and O (64 registers with wide
-// heads) is rarely rescaled. In front of the exponentials, `rescale` gets the factor where any row moves.
-template <int KB, typename F>
+// reference m, which follows the running maximum (less the lift) only when that has left it by more than 2^8: P and
+// the sums stay within 2^8 (and the lift) times the number of keys, nothing is lost in their floating types, and O (64
+// registers with wide heads) is rarely rescaled. In front of the exponentials, `rescale` gets the factor where any
+// row moves.
+template <typename E, int KB, typename F>
 __device__ __forceinline__ void soften(f32x16* s, float& m, float& l, float scale_log2, F&& rescale) {
   float mt = -INFINITY;
 #pragma unroll
@@ -313,8 +354,8 @@ __device__ __forceinline__ void soften(f32x16* s, float& m, float& l, float scal
 #pragma unroll
     for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
   mt = half_max(mt) * scale_log2;
-  if (__any(mt > m + 8.f)) {
-    const float mn = fmaxf(m, mt);
+  if (__any(mt > m + (8.f + kLift<E>))) {
+    const float mn = fmaxf(m, mt - kLift<E>);
     const float alpha = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
     l *= alpha;
     m = mn;
@@ -451,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
         for (int i = 0; i < 16; ++i)
           if (k0 + kb * 32 + acc_row(i, hh) >= k_end) s[kb][i] = -INFINITY;
     }
-    soften<2>(s, m, l, p.scale_log2, [&](float alpha) {
+    soften<E, 2>(s, m, l, p.scale_log2, [&](float alpha) {
 #pragma unroll
       for (int nb = 0; nb < L::NB; ++nb)
 #pragma unroll
@@ -542,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
       for (int i = 0; i < 16; ++i)
         if (k0 + acc_row(i, hh) >= k_end) s[i] = -INFINITY;
     }
-    soften<1>(&s, m, l, p.scale_log2, [&](float alpha) {
+    soften<E, 1>(&s, m, l, p.scale_log2, [&](float alpha) {
 #pragma unroll
       for (int nb = 0; nb < L::NB; ++nb)
 #pragma unroll
@@ -748,6 +789,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   f32x16 dq[L::NB];
 #pragma unroll
   for (int nb = 0; nb < L::NB; ++nb) dq[nb] = zero16();
+  Gain<E> gain;
   // S and dP of 32 keys, S turned into P; keys behind the end have P = 0
   auto scores = [&](const unsigned char* Ks, const unsigned char* Vs, int k0, int kb, f32x16& s, f32x16& dp) {
     s = zero16();
@@ -758,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
       dp = mfma<E>(lds.row8(Vs, kb * 32, st), df[st], dp);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse));
+    for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, kLiftBack<E> - lse));
     if (k0 + kb * 32 + 32 > k_end) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -768,6 +810,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   auto add = [&](const unsigned char* Ks, int kb, const f32x16& s, f32x16& dp) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - delta);
+    gain.fit(dp, dq);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const u16x8 db = to_operand<E>(dp, ks);
@@ -790,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += s[i] * dp[i];
       }
-      delta = half_sum(sum);
+      delta = half_sum(sum) * kUnliftBack<E>;
 #pragma unroll 1
       for (int kb = 0; kb < 2; ++kb) {
         scores(Ks, Vs, k0, kb, s, dp);
@@ -810,11 +853,12 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   }
   if (mine && hh == 0 && w.split == 0) p.delta[stat] = delta;
   if (!mine) return;
+  const float by = p.scale * gain.down();
   if (p.splits == 1) {
-    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4<E>(p.out + dense + col, dq[nb], i, p.scale); });
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4<E>(p.out + dense + col, dq[nb], i, by); });
   } else {
     float* at = p.part + w.split * p.out_numel + dense;
-    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4f(at + col, dq[nb], i, p.scale); });
+    each_quad<DP>(hh, p.D, [&](int col, int nb, int i) { put4f(at + col, dq[nb], i, by); });
   }
 }
 
@@ -859,6 +903,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   f32x16 dk[L::NB], dv[L::NB];
 #pragma unroll
   for (int nb = 0; nb < L::NB; ++nb) dk[nb] = dv[nb] = zero16();
+  Gain<E> gain;
   const bool second = Copy::second(wave);
   const int64_t H = (int64_t)p.N * p.G;
   const u16* base = second ? p.dout + w.b * (p.Tq * H * p.D) + (int64_t)w.n * p.G * p.D
@@ -906,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 4 * g4 + j;
-          const float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -ls[j]));
+          const float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, kLiftBack<E> - ls[j]));
           s[i] = pv;
           dp[i] = pv * (dp[i] - dl[j]);
         }
@@ -920,6 +965,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] = 0.f;
       }
+      gain.fit(dp, dk);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         const u16x8 pb = to_operand<E>(s, ks), db = to_operand<E>(dp, ks);
@@ -938,6 +984,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   if (key >= p.Tk) return;
   // a lane whose key lies behind the last state has been computing with zeros for its key: its columns are not used
   const bool live = key < len;
+  const float by = p.scale * gain.down();
   const int64_t at = (((int64_t)w.b * p.Tk + key) * 2 * p.N + w.n) * p.D, to_v = (int64_t)p.N * p.D;
   if (!live) {
 #pragma unroll
@@ -945,14 +992,14 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   }
   if (p.splits == 1) {
     each_quad<DP>(hh, p.D, [&](int col, int nb, int i) {
-      put4<E>(p.dkv + at + col, dk[nb], i, p.scale);
-      put4<E>(p.dkv + at + to_v + col, dv[nb], i, 1.f);
+      put4<E>(p.dkv + at + col, dk[nb], i, by);
+      put4<E>(p.dkv + at + to_v + col, dv[nb], i, kUnliftBack<E>);
     });
   } else {
     float* to = p.part + w.split * p.dkv_numel + at;
     each_quad<DP>(hh, p.D, [&](int col, int nb, int i) {
-      put4f(to + col, dk[nb], i, p.scale);
-      put4f(to + to_v + col, dv[nb], i, 1.f);
+      put4f(to + col, dk[nb], i, by);
+      put4f(to + to_v + col, dv[nb], i, kUnliftBack<E>);
     });
   }
 }

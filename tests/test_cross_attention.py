@@ -91,9 +91,9 @@ def _run(q, kv, do, lengths, scale=None):
     return {"o": o, "dq": dq, "dkv": dkv}
 
 
-def _hold(got, q, kv, do, lengths, scale=None):
+def _hold(got, q, kv, do, lengths, scale=None, tiny=None):
     ref, off = _reference(q, kv, do, lengths, q.shape[-1] ** -0.5 if scale is None else scale,
-                          torch.finfo(q.dtype).eps / 2, _tiny(q.dtype))
+                          torch.finfo(q.dtype).eps / 2, _tiny(q.dtype) if tiny is None else tiny)
     for k in ref:
         assert got[k].shape == ref[k].shape and got[k].dtype == q.dtype
         _check(k, got[k], ref[k], off[k])
@@ -198,6 +198,25 @@ def test_sharp_rows_and_another_scale(tq, g):
     dev = _cuda()
     q, kv, do = _inputs(dev, torch.bfloat16, 2, tq, 300, 4, g, 64, big=6.0)
     _hold(_run(q, kv, do, None, 0.3), q, kv, do, None, 0.3)
+
+
+@gpu
+def test_fp16_keeps_small_probabilities_and_large_gradients():
+    """A long source: each probability is far below fp16's normal range (2^-14), where half a step would be 2^-25. They
+    are lifted by 2^15, so that is 2^-40; dS by as much as its column's largest allows, so 2^-39 of that (under 8)."""
+    dev = _cuda()
+    q, kv, do = _inputs(dev, torch.float16, 1, 20, 30000, 2, 1, 64)
+    do = do * 64  # gradients in the normal range
+    _hold(_run(q, kv, do, None), q, kv, do, None, tiny=2.0 ** -36 * 64)
+    one = q.detach()[:, :1].clone().requires_grad_()
+    _hold(_run(one, kv, do[:, :1].contiguous(), None), one, kv, do[:, :1], None, tiny=2.0 ** -36 * 64)
+    # few states, large gradients of the output: dS beyond 65504, all results within it
+    q, kv, do = _inputs(dev, torch.float16, 1, 2, 3, 2, 1, 128, big=1e-3)
+    kv = (kv.detach() * torch.tensor([1.0, 2.0], device=dev).half()[:, None, None]).requires_grad_()
+    do = (do * 2e4).clamp(-6e4, 6e4)  # (3.3 standard deviations of them are beyond fp16)
+    got = _run(q, kv, do, None)
+    assert all(t.isfinite().all() for t in got.values())
+    _hold(got, q, kv, do, None)
 
 
 @gpu

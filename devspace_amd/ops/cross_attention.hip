@@ -117,6 +117,11 @@ template <typename E>
 constexpr float kLift = E::kType == at::kHalf ? 7.f : 0.f;
 template <typename E>
 constexpr float kLiftBack = E::kType == at::kHalf ? 15.f : 0.f;
+template <typename E>  // the exponent's constant (a negation costs an instruction nothing, a difference with 0 does)
+__device__ __forceinline__ float lift_back(float lse) {
+  if constexpr (E::kType == at::kHalf) return kLiftBack<E> - lse;
+  else return -lse;
+}
 template <typename E>
 constexpr float kUnliftBack = E::kType == at::kHalf ? 1.f / 32768.f : 1.f;
 
@@ -800,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
       dp = mfma<E>(lds.row8(Vs, kb * 32, st), df[st], dp);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, kLiftBack<E> - lse));
+    for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, lift_back<E>(lse)));
     if (k0 + kb * 32 + 32 > k_end) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -951,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 4 * g4 + j;
-          const float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, kLiftBack<E> - ls[j]));
+          const float pv = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, lift_back<E>(ls[j])));
           s[i] = pv;
           dp[i] = pv * (dp[i] - dl[j]);
         }
@@ -960,10 +965,6 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (r0 + qs * 32 + acc_row(i, hh) >= r_end) s[i] = dp[i] = 0.f;
-      }
-      if (len == 1) {  // a single state: dK = 0
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dp[i] = 0.f;
       }
       gain.fit(dp, dk);
 #pragma unroll
@@ -984,7 +985,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   if (key >= p.Tk) return;
   // a lane whose key lies behind the last state has been computing with zeros for its key: its columns are not used
   const bool live = key < len;
-  const float by = p.scale * gain.down();
+  const float by = len == 1 ? 0.f : p.scale * gain.down();  // the softmax of a single state is constant: dK = 0
   const int64_t at = (((int64_t)w.b * p.Tk + key) * 2 * p.N + w.n) * p.D, to_v = (int64_t)p.N * p.D;
   if (!live) {
 #pragma unroll

@@ -25,8 +25,8 @@
 //
 // What bounds it (MI355X, bf16; a large matrix product reaches 1367 TFLOP/s and a large copy 5.0 TB/s here):
 //   long rows      the matrix cores at the clock that the power allows (about 1.6 GHz then). 4 x 4096 x 4096, 16
-//                  heads of 128: forward 557 us (988 TFLOP/s), dQ 714 (1155), dK and dV 1046 (1051); all three
-//                  2121 us. Two kernels without atomics compute S and dP twice: 18 products' work for 14.
+//                  heads of 128: forward 568 us (968 TFLOP/s), dQ 733 (1125), dK and dV 1084 (1014); all three,
+//                  among others, 2189 us. Two kernels without atomics compute S and dP twice: 18 products' work for 14.
 //                  16 heads of 64: forward 335 us (821), dQ 405 (1018), dK and dV 609 (903): the exponentials and
 //                  sums of a tile take as long as its products.
 //   short rows     latency of a tile and of a launch: 8 x 512 x 512 ragged, 16 heads of 64: 18, 23 and 28 us

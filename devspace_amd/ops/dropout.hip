@@ -16,9 +16,9 @@
 // types) are two blocks whatever the row's length. All of a row's math is in fp32; each output is rounded
 // once, and y is made of the sum before its rounding.
 //
-// Bound by memory, the generator's work hidden behind it. MI355X: 32768 x 8192 bf16 forward and backward 372 us
-// (5.8 TB/s, a large copy reaches 5.0); 4096 x 1024 bf16 add + norm 10.7 us forward (3.1 TB/s), 12.7 + 3.9 us
-// backward (3.3 TB/s), a few us of each being the launch; 4095 x 1023 fp16 7.3 us a pass.
+// Bound by memory, the generator's work hidden behind it. MI355X: 32768 x 8192 bf16 forward and backward 381 us
+// (5.6 TB/s, a large copy reaches 5.0); 4096 x 1024 bf16 add + norm 9.8 us forward (3.4 TB/s), 14.0 + 3.9 us
+// backward (3.6 TB/s), a few us of each being the launch; 4095 x 1023 fp16 7.2 us a pass.
 #include "fused_common.h"
 
 #include <algorithm>

@@ -10,7 +10,7 @@
 // sines and cosines once into LDS and uses them for every head of q, k (and the packed v's copy), so
 // their cost shrinks with the number of heads and any position works. Bound by memory: each element is
 // read once and written once, in accesses of up to 16 bytes, neighbouring lanes on neighbouring
-// columns and heads of a token. MI355X: 32749 tokens x 40 heads x 128 bf16, 125 us a pass (5.4 TB/s, a large
+// columns and heads of a token. MI355X: 32749 tokens x 40 heads x 128 bf16, 126 us a pass (5.3 TB/s, a large
 // copy reaches 5.0); 8 x 512 packed tokens x 16 heads x 64, 12 us; 16 single tokens 4 us, a launch's latency.
 #include "fused_common.h"
 

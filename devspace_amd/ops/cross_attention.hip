@@ -30,7 +30,7 @@
 //                  16 heads of 64: forward 335 us (821), dQ 405 (1018), dK and dV 609 (903): the exponentials and
 //                  sums of a tile take as long as its products.
 //   short rows     latency of a tile and of a launch: 8 x 512 x 512 ragged, 16 heads of 64: 18, 23 and 28 us
-//   single tokens  memory: 32 tokens over 1500 ragged states, 16 heads of 64: 39 us (3.8 TB/s); one token over
+//   single tokens  memory: 32 tokens over 1500 ragged states, 16 heads of 64: 37 us (4.0 TB/s); one token over
 //                  131071 states, 8 key heads of 128: 104 us with its join (5.2 TB/s)
 #include "fused_common.h"
 
@@ -188,18 +188,26 @@ struct CrossParams {
   }
 };
 
-// Which work a workgroup has. Workgroups go to the 8 XCDs in turn; the ones of one key head (neighbours here)
-// are given to one XCD, whose L2 then serves its keys and values.
+// Which work a workgroup has. Workgroups go to the 8 XCDs in turn; all of one key head are given to one XCD, whose L2
+// then serves its keys and values, and neighbouring heads to different XCDs, so that sequences of unlike lengths are
+// spread evenly (8 ragged sequences of 16 heads, trained: 62.2 us, with one sequence to an XCD 65.2; 32 single tokens
+// 37.2 us for 39.1).
 struct Place {
   int block, split, n, b, bn;
   __device__ __forceinline__ explicit Place(const CrossParams& p) {
-    const unsigned total = gridDim.x, id = blockIdx.x;
-    const unsigned xcd = id & 7, slot = id >> 3, each = total >> 3, rest = total & 7;
-    unsigned w = xcd * each + min(xcd, rest) + slot;
-    block = w % p.blocks;
-    w /= p.blocks;
-    split = w % p.splits;
-    bn = w / p.splits;
+    const unsigned id = blockIdx.x, each = p.blocks * p.splits, even = (unsigned)(p.B * p.N) & ~7u;
+    unsigned rest;
+    if (id < even * each) {
+      const unsigned slot = id >> 3;
+      bn = (int)(slot / each * 8 + (id & 7));
+      rest = slot % each;
+    } else {  // up to 7 heads more, in turn
+      const unsigned over = id - even * each;
+      bn = (int)(even + over / each);
+      rest = over % each;
+    }
+    block = rest % p.blocks;
+    split = rest / p.blocks;
     n = bn % p.N;
     b = bn / p.N;
   }
@@ -529,8 +537,8 @@ __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
   }
 }
 
-// Up to 32 rows: wave w takes the 32-key tiles w, w + 4, ... of the split. Bound by memory: with the loads of two
-// tiles under way per wave (heads of 64), 32 tokens over 1500 states take 39 us, with one 45 us.
+// Up to 32 rows: wave w takes the 32-key tiles w, w + 4, ... of the split. Bound by memory: the loads of two
+// tiles are under way per wave (heads of 64; with one, 32 tokens over 1500 states took 45 us for 39).
 template <typename E, int DP>
 __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   typedef Tile<DP> L;

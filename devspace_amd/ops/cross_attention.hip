@@ -1217,7 +1217,7 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "cross_attention: second derivatives are not implemented");
+    no_second_order("cross_attention");
     auto s = ctx->get_saved_variables();
     OptTensor lengths;
     if (s[4].defined()) lengths = s[4];
@@ -1231,6 +1231,7 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
 
 at::Tensor cross_attention(const at::Tensor& q, const at::Tensor& kv, const OptTensor& lengths, double scale) {
   const char* op = "cross_attention: ";
+  no_tangents("cross_attention", q, kv);
   TORCH_CHECK(q.is_cuda() && kv.device() == q.device(), op, "q and kv must be on one GPU");
   TORCH_CHECK(q.scalar_type() == kv.scalar_type() && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf), op,
               "q and kv must both be bfloat16 or float16");

@@ -527,10 +527,6 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 typedef c10::optional<at::Tensor> OptTensor;
 
-void no_second_order(const char* op) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": second derivatives are not implemented");
-}
-
 void save_drop(AutogradContext* ctx, double p, int64_t seed, int64_t offset) {
   ctx->saved_data["p"] = p;
   ctx->saved_data["seed"] = seed;
@@ -582,6 +578,7 @@ struct DropNormFn : public torch::autograd::Function<DropNormFn> {
 at::Tensor dropout(const at::Tensor& d, const OptTensor& x, double p, int64_t seed, const OptTensor& seed_at,
                    int64_t offset) {
   const char* op = x ? "dropout_add" : "dropout";
+  no_tangents(op, d, or_none(x));
   check_drop(op, d, p, seed_at, offset);
   if (x) same(op, "x and delta", *x, d);
   if (at::GradMode::is_enabled() && (d.requires_grad() || (x && x->requires_grad())))
@@ -592,6 +589,7 @@ at::Tensor dropout(const at::Tensor& d, const OptTensor& x, double p, int64_t se
 std::vector<at::Tensor> dropout_add_rms_norm(const at::Tensor& x, const at::Tensor& delta, const at::Tensor& w, double eps,
                                              double p, int64_t seed, const OptTensor& seed_at, int64_t offset) {
   const char* op = "dropout_add_rms_norm";
+  no_tangents(op, x, delta, w);
   check_drop(op, x, p, seed_at, offset);
   same(op, "x and delta", x, delta);
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) <= kMaxNormDim, op, ": rows of at most ", kMaxNormDim, " elements wanted");

@@ -37,6 +37,18 @@ inline hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }
     TORCH_CHECK(e_ == hipSuccess, "HIP launch failed: ", hipGetErrorString(e_));               \
   } while (0)
 
+// What the operators without derivatives of derivatives refuse. A backward pass that is itself to be differentiated:
+inline void no_second_order(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": second derivatives are not implemented");
+}
+// A tangent of forward mode on any input: it needs no requires_grad, so that a call could pass the autograd node by,
+// compute the value alone and lose the tangent without a word. Checked in front of all else.
+template <typename... Tensors>
+inline void no_tangents(const char* op, const Tensors&... inputs) {
+  TORCH_CHECK(!(inputs._fw_grad(0).defined() || ...), op, ": forward-mode derivatives are not implemented");
+}
+inline at::Tensor or_none(const c10::optional<at::Tensor>& t) { return t ? *t : at::Tensor(); }
+
 // ------------------------------------------------------------------------------ element types
 // Storage of one element and its way to and from fp32 (round to nearest even).
 struct BF16 {

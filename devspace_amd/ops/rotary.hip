@@ -287,10 +287,6 @@ void check_rotary(const at::Tensor& x, const char* name, const at::Tensor& freq)
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-void no_second_order(const char* op) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": second derivatives are not implemented");
-}
-
 struct RotaryFn : public torch::autograd::Function<RotaryFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const c10::optional<at::Tensor>& k, bool packed,
                                const c10::optional<at::Tensor>& pos, int64_t start, const at::Tensor& freq,
@@ -324,6 +320,7 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
 std::vector<at::Tensor> rotary(const at::Tensor& q, const c10::optional<at::Tensor>& k, bool packed,
                                const c10::optional<at::Tensor>& pos, int64_t start, const at::Tensor& freq,
                                bool interleaved, double magnitude) {
+  no_tangents("rotary", q, or_none(k), freq);
   check_rotary(q, packed ? "qkv" : "q", freq);
   TORCH_CHECK(q.dim() == (packed ? 5 : 4) && (!packed || q.size(2) == 3), "rotary: ",
               packed ? "qkv must be [B, T, 3, H, D]" : "heads must be [B, T, H, D]");

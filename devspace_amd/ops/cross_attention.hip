@@ -786,7 +786,8 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   const Places<DP> lds(lane);
   const int m0 = w.block * kRows + wave * 32, row = m0 + r;
   const bool some = m0 < p.M, mine = row < p.M;
-  const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
+  const int len = p.length(w.b);
+  const int k_begin = w.split * p.per_split, k_end = min(len, k_begin + p.per_split);
   const int64_t dense = mine ? p.dense_at(row, w.b, w.n) : 0, stat = (int64_t)w.bn * p.M + row;
   u16x8 qf[L::KS], df[L::KS];
   load_row<DP>(df, mine ? p.dout + dense : nullptr, hh, p.D);
@@ -831,9 +832,11 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
       for (int nb = 0; nb < L::NB; ++nb) dq[nb] = mfma<E>(lds.tr8(Ks, kb * 32 + 16 * ks, nb), db, dq[nb]);
     }
   };
-  if (p.splits == 1 && k_end <= 1) {
+  // By the sequence's own length, not by the launch: the first part of a split axis holds four tiles at least, so all
+  // of a short sequence, and the others have none of it.
+  if (len <= 1) {
     // the softmax of a single state is constant: dQ = 0, and nothing of P's last bits in it
-  } else if (p.splits == 1 && k_end <= kKeys) {
+  } else if (len <= kKeys) {
     // One tile holds all states. With few of them, the rounding of O weighs in dO . O, which nearly equals the
     // dP it is taken from; here it is summed from P and dP themselves.
     key_loop<DP>(tile0, tile1, tile2, p, w, wave, lane, k_begin, k_end, [&](const unsigned char* Ks, const unsigned char* Vs, int k0) {

@@ -396,3 +396,66 @@ def test_captured_with_lengths_read_at_each_replay():
         torch.cuda.synchronize()
         for a, b in zip(outs, step()):
             assert torch.equal(a, b)
+
+
+def _short_reference(q, kv, do, lengths, scale, h_step, tiny):
+    """_reference's gradients of sequences of 1 to 64 states, where the row sum is taken from the unrounded P and dP, in
+    32 bits: it is off by P's share and dP's of each of its terms and by (m + 8) u of their sizes, not by O's
+    rounding. A single state's dQ and dK are 0 exactly."""
+    q, kv, do = (t.detach().double().cpu() for t in (q, kv, do))
+    b, tq, hh, d = q.shape
+    grp = hh // kv.shape[3]
+    dq, dkv = torch.zeros_like(q), torch.zeros_like(kv)
+    off_q, off_kv = torch.zeros_like(q), torch.zeros_like(kv)
+    for i, m in enumerate(lengths):
+        for j in range(hh if m else 0):
+            k, v = kv[i, :m, 0, j // grp], kv[i, :m, 1, j // grp]
+            x, y = q[i, :, j], do[i, :, j]
+            p = torch.softmax(scale * (x @ k.T), -1)
+            e_p = 2 * (d + 8) * U * (scale * (x.abs() @ k.abs().T)).amax(-1, keepdim=True) + (m + 16) * U
+            steps = (max(m, tq * grp) + 16) * U
+            dkv[i, :m, 1, j // grp] += p.T @ y
+            off_kv[i, :m, 1, j // grp] += ((h_step + e_p + steps) * p + tiny).T @ y.abs() + tiny * tq
+            if m == 1:
+                continue
+            dp = y @ v.T
+            e_dp = (d + 2) * U * (y.abs() @ v.abs().T)
+            row = (p * dp).sum(-1, keepdim=True)
+            e_row = (p * ((e_p + (m + 8) * U) * dp.abs() + e_dp)).sum(-1, keepdim=True)
+            ds = p * (dp - row)
+            e_ds = h_step * ds.abs() + (1 + h_step) * p * (e_p * (dp - row).abs() + e_dp + e_row) + tiny * ((dp - row).abs() + 1)
+            dq[i, :, j] = scale * ds @ k
+            off_q[i, :, j] = scale * ((e_ds + steps * ds.abs()) @ k.abs() + tiny * m)
+            dkv[i, :m, 0, j // grp] += scale * ds.T @ x
+            off_kv[i, :m, 0, j // grp] += scale * ((e_ds + steps * ds.abs()).T @ x.abs() + tiny * tq)
+    return {"dq": (dq, off_q), "dkv": (dkv, off_kv)}
+
+
+@gpu
+@pytest.mark.parametrize("dtype,b,tq,tk,h,g,d,lengths,big", [
+    ("bf16", 5, 40, 1500, 2, 1, 64, (1500, 1, 2, 64, 0), 1.0),
+    ("bf16", 4, 17, 1500, 4, 4, 128, (1, 63, 3, 1499), 4.0),
+    ("fp16", 3, 1, 6000, 2, 2, 80, (2, 1, 33), 1.0),
+    ("fp16", 3, 300, 770, 1, 1, 96, (1, 5, 64), 4.0),
+    ("bf16", 3, 40, 64, 2, 1, 64, (2, 1, 64), 4.0),  # one tile, for comparison: no split
+])
+def test_short_sources_beside_long_ones(dtype, b, tq, tk, h, g, d, lengths, big):
+    """How exact a sequence's gradients are goes by its own length: a long axis beside it, for which the launch is split,
+    changes nothing."""
+    dev = _cuda()
+    q, kv, do = _inputs(dev, DTYPES[dtype], b, tq, tk, h, g, d, big=big)
+    n = torch.tensor(lengths, device=dev)
+    got = _run(q, kv, do, n)
+    _hold(got, q, kv, do, n)
+    short = [i for i, m in enumerate(lengths) if m <= 64]
+    ref = _short_reference(q[short], kv[short], do[short], [lengths[i] for i in short], d ** -0.5,
+                           torch.finfo(q.dtype).eps / 2, _tiny(q.dtype))
+    for k, (want, off) in ref.items():
+        _check(k, got[k][short], want, off)
+    for i in short:
+        if lengths[i] <= 1:
+            assert not got["dq"][i].any() and not got["dkv"][i, :, 0].any()
+    # the same bits as with nothing but its first 64 states around it
+    alone = _run(q, kv.detach()[:, :64].clone().requires_grad_(), do, n.clamp(max=64))
+    for i in short:
+        assert torch.equal(alone["dq"][i], got["dq"][i]) and torch.equal(alone["dkv"][i], got["dkv"][i, :64])

@@ -176,6 +176,12 @@ struct CrossParams {
   }
   // the same for a sequence that all lanes share
   __device__ __forceinline__ int length(int b) const { return __builtin_amdgcn_readfirstlane(length_of(b)); }
+  // Axes come near to 2^31, where begin + per_split does not fit 32 bits: where a split ends, and how many have any of
+  // an axis' first len.
+  __device__ __forceinline__ int split_end(int begin, int len) const { return begin + min(per_split, len - begin); }
+  __device__ __forceinline__ int parts_of(int len) const {
+    return (int)(((unsigned)len + (unsigned)per_split - 1u) / (unsigned)per_split);
+  }
   // offset of row m of key head n in [B, Tq, H, D] with these strides
   __device__ __forceinline__ int64_t row_at(int m, int b, int n, int64_t sb, int64_t st, int64_t sh) const {
     unsigned g;
@@ -484,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_fwd_kernel(CrossParams p) {
   const Places<DP> lds(lane);
   const int m0 = w.block * kRows + wave * 32, row = m0 + r;
   const bool some = m0 < p.M;  // the wave has rows at all
-  const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
+  const int k_begin = w.split * p.per_split, k_end = p.split_end(k_begin, p.length(w.b));
   u16x8 qf[L::KS];
   load_row<DP>(qf, row < p.M ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
   f32x16 o[L::NB];
@@ -555,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   const Places<DP> lds(lane);
   const int m0 = w.block * 32, row = m0 + r;
   const int rows = min(32, p.M - m0);
-  const int k_begin = w.split * p.per_split, k_end = min(p.length(w.b), k_begin + p.per_split);
+  const int k_begin = w.split * p.per_split, k_end = p.split_end(k_begin, p.length(w.b));
   const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh;
   u16x8 qf[L::KS];
   load_row<DP>(qf, row < p.M ? p.q + p.row_at(row, w.b, w.n, p.qb, p.qt, p.qh) : nullptr, hh, p.D);
@@ -575,9 +581,10 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   struct Keys {  // one tile on its way: keys as operands, values by rows
     u16x8 k[L::KS], v[kPer];
   };
-  auto load = [&](Keys& t, int k0) {
-    const u16* base = kbase + (k0 < k_end ? k0 : 0) * p.kt;
-    const unsigned bytes = bytes_of(k_end - k0, p.kt, p.D);
+  auto load = [&](Keys& t, unsigned k0) {  // positions past the end pass 2^31, too
+    const bool any = k0 < (unsigned)k_end;
+    const u16* base = kbase + (any ? k0 : 0u) * p.kt;
+    const unsigned bytes = any ? bytes_of((int)((unsigned)k_end - k0), p.kt, p.D) : 0u;
     to_registers(t.k, base, bytes, at_k);
     to_registers(t.v, base + p.ks, bytes, at_v);
   };
@@ -590,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
       const int c = lane + 64 * u;
       *reinterpret_cast<u16x8*>(Vs + L::off(c / L::CH, c % L::CH)) = t.v[u];
     }
-    load(t, k0 + ahead);
+    load(t, (unsigned)k0 + ahead);
     if (k0 + kTile > k_end) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -622,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_few_kernel(CrossParams p) {
   Keys t0, t1;
   load(t0, k0);
   if constexpr (L::BUFS == 3) {
-    load(t1, k0 + kStride);
+    load(t1, (unsigned)k0 + kStride);
     while (k0 < k_end) {
       step(t0, k0, 2 * kStride);
       if ((k0 += kStride) >= k_end) break;
@@ -690,8 +697,7 @@ __global__ void __launch_bounds__(kThreads) cross_join_many_kernel(CrossParams p
   const int col = (int)quad * 4;
   const int bn = (int)(stat / (unsigned)p.M), row = (int)(stat - (unsigned)bn * p.M);
   const int b = bn / p.N, n = bn - b * p.N;
-  const int len = p.length_of(b);
-  const int parts = (len + p.per_split - 1) / p.per_split;
+  const int parts = p.parts_of(p.length_of(b));
   const int64_t step = (int64_t)p.B * p.N * p.M;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + stat;
   float m = -INFINITY;
@@ -723,7 +729,7 @@ __global__ void __launch_bounds__(THREADS) cross_join_kernel(CrossParams p) {
   const int64_t stat = blockIdx.x;  // bn M + row
   const int bn = (int)(stat / p.M), row = (int)(stat - (int64_t)bn * p.M);
   const int b = bn / p.N, n = bn - b * p.N;
-  const int parts = (p.length(b) + p.per_split - 1) / p.per_split;
+  const int parts = p.parts_of(p.length(b));
   const int64_t step = (int64_t)p.B * p.N * p.M;
   const int wave = threadIdx.x >> 6;
   float m = -INFINITY;
@@ -787,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dq_kernel(CrossParams p) {
   const int m0 = w.block * kRows + wave * 32, row = m0 + r;
   const bool some = m0 < p.M, mine = row < p.M;
   const int len = p.length(w.b);
-  const int k_begin = w.split * p.per_split, k_end = min(len, k_begin + p.per_split);
+  const int k_begin = w.split * p.per_split, k_end = p.split_end(k_begin, len);
   const int64_t dense = mine ? p.dense_at(row, w.b, w.n) : 0, stat = (int64_t)w.bn * p.M + row;
   u16x8 qf[L::KS], df[L::KS];
   load_row<DP>(df, mine ? p.dout + dense : nullptr, hh, p.D);
@@ -902,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 2) cross_dkv_kernel(CrossParams p) {
   const bool some = kw < len;
   // a block of keys behind the last state has no work but its zeros
   const int r_begin = w.split * p.per_split;
-  const int r_end = w.block * kRows < len ? min(p.M, r_begin + p.per_split) : r_begin;
+  const int r_end = w.block * kRows < len ? p.split_end(r_begin, p.M) : r_begin;
   const u16* kbase = p.kv + w.b * p.kb + w.n * p.kh + (int64_t)key * p.kt;
   u16x8 kf[L::KS], vf[kVInLds ? 1 : L::KS];
   load_row<DP>(kf, key < len ? kbase : nullptr, hh, p.D);

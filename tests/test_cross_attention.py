@@ -459,3 +459,57 @@ def test_short_sources_beside_long_ones(dtype, b, tq, tk, h, g, d, lengths, big)
     alone = _run(q, kv.detach()[:, :64].clone().requires_grad_(), do, n.clamp(max=64))
     for i in short:
         assert torch.equal(alone["dq"][i], got["dq"][i]) and torch.equal(alone["dkv"][i], got["dkv"][i, :64])
+
+
+@gpu
+@pytest.mark.parametrize("tk", [(1 << 31) - 1_000_000, (1 << 31) - 129])
+@pytest.mark.parametrize("tq", [1, 33])
+def test_almost_two_to_the_31_states(tk, tq):
+    """Sums of positions that pass 32 bits: where parts end, how many parts there are, tiles fetched ahead. The last two
+    states have equal scores of 1018, the others 0: their probabilities are 0 in 32 bits, together too (2^31 e^-1018)."""
+    dev = _cuda()
+    if torch.cuda.get_device_properties(0).total_memory < 200 << 30:
+        pytest.skip("needs 140 GB for the states and their gradients")
+    torch.cuda.empty_cache()
+    kv = torch.zeros(1, tk, 2, 1, 8, device=dev, dtype=torch.bfloat16)
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(1)
+    kv[0, -2:, 0, 0] = torch.tensor([[120.0] * 8, [240.0, 0.0] * 4], device=dev).bfloat16()
+    kv[0, -2:, 1] = torch.randn(2, 1, 8, device=dev, generator=gen).bfloat16()
+    q = torch.full((1, tq, 1, 8), 3.0, device=dev, dtype=torch.bfloat16).requires_grad_()
+    do = torch.randn(1, tq, 1, 8, device=dev, generator=gen).bfloat16()
+    last = kv[:, -2:].clone()
+    o = fused.cross_attention(q, kv.requires_grad_())
+    dq, dkv = torch.autograd.grad(o, (q, kv), do)
+    _hold({"o": o, "dq": dq, "dkv": dkv[:, -2:]}, q, last, do, None)
+    assert dq.any() and not dkv[:, :-2].any()
+    # a source that ends where the parts of its axis are being counted
+    n = torch.tensor([tk - 1], device=dev)
+    with torch.no_grad():
+        assert torch.equal(fused.cross_attention(q, kv, n), last[:, :1, 1].expand(1, tq, 1, 8))
+    del kv, dkv
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_almost_two_to_the_31_rows():
+    """The same for the rows, over which dK and dV are split: only the last rows have a gradient."""
+    dev = _cuda()
+    if torch.cuda.get_device_properties(0).total_memory < 200 << 30:
+        pytest.skip("needs 160 GB for the rows and their gradients")
+    torch.cuda.empty_cache()
+    rows = (1 << 31) - 129
+    q = torch.zeros(1, rows, 1, 8, device=dev, dtype=torch.bfloat16)
+    do = torch.zeros_like(q)
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(1)
+    q[:, -9:] = torch.randn(1, 9, 1, 8, device=dev, generator=gen).bfloat16()
+    do[:, -9:] = torch.randn(1, 9, 1, 8, device=dev, generator=gen).bfloat16()
+    kv = torch.randn(1, 5, 2, 1, 8, device=dev, generator=gen).bfloat16().requires_grad_()
+    last, grad = q[:, -9:].clone(), do[:, -9:].clone()
+    o = fused.cross_attention(q.requires_grad_(), kv)
+    dq, dkv = torch.autograd.grad(o, (q, kv), do)
+    _hold({"o": o[:, -9:], "dq": dq[:, -9:], "dkv": dkv}, last, kv, grad, None)
+    assert not dq[:, :-9].any()
+    del q, do, o, dq
+    torch.cuda.empty_cache()

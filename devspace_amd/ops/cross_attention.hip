@@ -1066,7 +1066,9 @@ void split_axis(CrossParams& p, int64_t have, int len, int tile) {
 
 unsigned grid_of(const CrossParams& p) {
   const int64_t g = (int64_t)p.blocks * p.splits * p.B * p.N;
-  TORCH_CHECK(g < (1ll << 24), "cross_attention: fewer than 2^24 workgroups wanted (sequences x key heads x blocks of 128)");
+  TORCH_CHECK(g < (1ll << 24),
+              "cross_attention: fewer than 2^24 workgroups wanted (sequences x key heads x blocks of 128 rows; for the states' "
+              "gradient blocks of 128 states)");
   return (unsigned)g;
 }
 

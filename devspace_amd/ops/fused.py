@@ -195,7 +195,8 @@ def cross_attention(q: torch.Tensor, kv: torch.Tensor, lengths: torch.Tensor | N
     gradients are 0; a sequence of no states gives 0. Any strides; Tq and Tk of any length, one query token
     included (serving). bfloat16 and float16 run the gfx950 kernels on a GPU (MFMA, forward and backward),
     with D a multiple of 8 up to 128, H times D up to 2^20 and fewer than 2^24 blocks (one per sequence, key head
-    and 128 stacked query rows); float32 and float64 are computed in PyTorch ops."""
+    and 128 stacked query rows; the backward pass for kv, one per 128 states); float32 and float64 are computed in
+    PyTorch ops."""
     if q.dim() != 4 or kv.dim() != 5 or kv.shape[2] != 2:
         raise ValueError("cross_attention: q must be [B, Tq, H, D] and kv [B, Tk, 2, N, D]")
     b, _, h, d = q.shape

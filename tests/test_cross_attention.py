@@ -513,3 +513,19 @@ def test_almost_two_to_the_31_rows():
     assert not dq[:, :-9].any()
     del q, do, o, dq
     torch.cuda.empty_cache()
+
+
+@gpu
+def test_more_blocks_of_states_than_a_launch_takes():
+    """2^24 blocks of 128 states, all of one source, so that the call itself is small: the states' gradient is refused,
+    the rest is not."""
+    dev = _cuda()
+    source = torch.ones(1, 1 << 19, 2, 1, 8, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    q = torch.ones(1 << 12, 1, 1, 8, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    o = fused.cross_attention(q, source.expand(1 << 12, -1, -1, -1, -1))
+    assert torch.equal(o, q)
+    (dq,) = torch.autograd.grad(o.sum(), q, retain_graph=True)
+    # V is constant: dS is P times what O's rounding and two sums of 8 products leave, its sum with K = 1 no more
+    assert not dq.float().abs().max() > 2 * 8 * 2.0 ** -8
+    with pytest.raises(RuntimeError, match="blocks of 128 states"):
+        torch.autograd.grad(o.sum(), source)

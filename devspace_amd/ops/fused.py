@@ -468,7 +468,7 @@ class Dropout(nn.Module):
     def forward(self, x, residual=None):
         if not self.training or self.p == 0.0:
             return x if residual is None else residual + x
-        seed = int(torch.randint(-(1 << 63), (1 << 63) - 1, ()))
+        seed = int(torch.randint(-(1 << 63), (1 << 63) - 1, (), device="cpu"))  # whatever the default device is
         return dropout(x, self.p, seed) if residual is None else dropout_add(residual, x, self.p, seed)
 
 

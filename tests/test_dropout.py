@@ -306,3 +306,33 @@ def test_norm_of_more_rows_than_one_launch_takes():
         assert torch.equal(s[row].double().cpu(), want), row
         ref = want * want.square().mean().rsqrt()
         assert ((y[row].double().cpu() - ref).abs() <= 1.01 * 2.0 ** -8 * ref).all(), row
+
+
+def test_module_draws_from_the_cpu_generator_whatever_the_default_device():
+    """On a GPU as default device the seed would come from the GPU's generator, and the call would wait for it; on
+    `meta` there is none to draw from."""
+    m, x = fused.Dropout(0.5), torch.randn(4, 64)
+    torch.manual_seed(5)
+    want = m(x)
+    torch.manual_seed(5)
+    with torch.device("meta"):
+        seed_of_the_call = []
+        real = fused.dropout
+        fused.dropout = lambda t, p, seed, offset=0: seed_of_the_call.append(seed)
+        try:
+            m(x)
+        finally:
+            fused.dropout = real
+    assert torch.equal(fused.dropout(x, 0.5, seed_of_the_call[0]), want)
+
+
+@gpu
+def test_module_draws_from_the_cpu_generator_with_a_gpu_as_default_device():
+    dev = _cuda()
+    m, x = fused.Dropout(0.5), torch.randn(4, 64, device=dev)
+    torch.manual_seed(5)
+    want = m(x)
+    torch.cuda.manual_seed(99)  # another state of the GPU's generator changes nothing
+    torch.default_generator.manual_seed(5)
+    with dev:
+        assert torch.equal(m(x), want)

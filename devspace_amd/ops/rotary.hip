@@ -194,7 +194,7 @@ void launch_rotary(RotaryParams& p, bool interleaved, hipStream_t st) {
   p.by_T = FastDiv((unsigned)p.T);
   p.by_half = FastDiv((unsigned)half);
   const int64_t blocks = (p.tokens + tb - 1) / tb;
-  TORCH_CHECK(blocks < (1ll << 31), "rotary: too many tokens");
+  TORCH_CHECK(blocks < (1ll << 32) / kThreads, "rotary: too many tokens for one launch of fewer than 2^32 work items");
   const size_t lds = (size_t)tb * 2 * p.pad * sizeof(float);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), lds, st, p); };
 #define ROTARY_CASE(W)                                                                        \

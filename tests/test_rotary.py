@@ -277,3 +277,13 @@ def test_captured_and_replayed_on_another_stream():
         assert torch.equal(yq, eq) and torch.equal(yk, ek)
         for a, b in zip(trained, train()):
             assert torch.equal(a, b)
+
+
+@gpu
+def test_more_tokens_than_one_launch_takes():
+    """2^24 blocks of 256 threads are 2^32 work items, one more than a launch holds: refused by name."""
+    dev = _cuda()
+    f = fused.rotary_frequencies(2, device=dev)[0]
+    x = torch.ones(1, 1, 1, 2, device=dev, dtype=torch.bfloat16).expand(3, 1_500_000_000, 1, 2)
+    with pytest.raises(RuntimeError, match="rotary: too many tokens"):
+        fused.rotary(x, 0, f)

@@ -140,3 +140,61 @@ def test_two_streams_at_once():
         for a, b in zip(want, got):
             for x, y in zip(a, b):
                 assert torch.equal(x, y)
+
+
+# A rounding to bf16 is off by at most 2^-8 of a value, evenly spread, so by 2^-8 / sqrt(3) in the mean square. Roundings
+# of different tensors are independent: k of them, each passed on by a norm of about one, are off by sqrt(k) times that.
+# Twice that is allowed, for the steps that pass on a little more (norms of rows shorter than the mean, softmax).
+def _independent(k):
+    return 2 * k ** 0.5 * 2.0 ** -8 / 3 ** 0.5
+
+
+def _train_at(p, dtype, device):
+    w = _weights(dtype, device)
+    x, states, g, lengths, freqs = _inputs(dtype, device)
+    y = _block(w, x, states, lengths, freqs, p=p)
+    leaves = {"x": x, "states": states, **w}
+    grads = torch.autograd.grad(y, list(leaves.values()), g)
+    return {"y": y, **{"d" + k: v for k, v in zip(leaves, grads)}}
+
+
+HALF = 0.5  # a lost 1 / (1 - p) is a factor of two
+
+
+class _Unscaled(torch.autograd.Function):
+    """x, and for its gradient (1 - p) times what it should be."""
+
+    @staticmethod
+    def forward(ctx, x, share):
+        ctx.share = share
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return g * ctx.share, None
+
+
+@pytest.mark.parametrize("where,leaf", [(0, "dproj"), (1, "dout"), (2, "ddown")])
+def test_a_lost_scale_is_beyond_what_roundings_explain(where, leaf, monkeypatch):
+    """The bound of the test below tells a wrong backward pass: 1 / (1 - p) left out of one dropout's gradient, planted
+    in the 64-bit form."""
+    want = _train_at(HALF, torch.float64, "cpu")
+    real = fused._dropped
+    monkeypatch.setattr(fused, "_dropped", lambda x, p, seed, at, offset: real(
+        _Unscaled.apply(x, 1 - p) if offset == where else x, p, seed, at, offset))
+    got = _train_at(HALF, torch.float64, "cpu")
+    assert torch.equal(got["y"], want["y"])
+    assert _off(got[leaf], want[leaf]) > 10 * _independent(42)
+
+
+@gpu
+@pytest.mark.parametrize("p", [P, HALF])
+def test_block_trains_within_independent_roundings(p):
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    fused.ext()
+    got, want = _train_at(p, torch.bfloat16, "cuda"), _train_at(p, torch.float64, "cpu")
+    for k in want:
+        off = _off(got[k], want[k])
+        print(f"{k} {off:.5f}")
+        assert off < _independent(14 if k == "y" else 42), (k, off)

@@ -24,11 +24,12 @@
 // buffer loads that write LDS without passing registers, one or two tiles ahead of their use, one barrier a tile.
 //
 // What bounds it (MI355X, bf16; a large matrix product reaches 1367 TFLOP/s and a large copy 5.0 TB/s here):
-//   long rows      the matrix cores at the clock that the power allows (about 1.6 GHz then). 4 x 4096 x 4096, 16
-//                  heads of 128: forward 568 us (968 TFLOP/s), dQ 733 (1125), dK and dV 1084 (1014); all three,
-//                  among others, 2189 us. Two kernels without atomics compute S and dP twice: 18 products' work for 14.
-//                  16 heads of 64: forward 335 us (821), dQ 405 (1018), dK and dV 609 (903): the exponentials and
-//                  sums of a tile take as long as its products.
+//   long rows      no unit alone: what a wave does between its products (softmax, conversions, LDS reads) is hidden in
+//                  part only. 4 x 4096 x 4096, 16 heads of 128: forward 509 us (1080 TFLOP/s), dQ 692 (1192), dK and dV
+//                  967 (1137), all three among others 2182; the matrix cores are busy in 54, 63 and 57 % of the cycles,
+//                  at 1.8 to 1.9 GHz, LDS conflicts in 0.1 % at the most. Two kernels without atomics compute S and dP
+//                  twice: 18 products' work for 14. 16 heads of 64, with as many exponentials for half of the products:
+//                  299 us (919), 386 (1068), 521 (1055), matrix cores busy in 45, 57 and 52 %.
 //   short rows     latency of a tile and of a launch: 8 x 512 x 512 ragged, 16 heads of 64: 18, 23 and 28 us
 //   single tokens  memory: 32 tokens over 1500 ragged states, 16 heads of 64: 37 us (4.0 TB/s); one token over
 //                  131071 states, 8 key heads of 128: 104 us with its join (5.2 TB/s)

@@ -9,9 +9,11 @@
     x, h = fused.dropout_add_rms_norm(x, delta, norm.weight, p, seed)  # no mask is stored
     o = fused.cross_attention(q, kv, lengths)         # over an encoder's states of another length
 
-On a GPU the HIP kernels are mandatory: if the in-tree extension is missing or broken the
-first call raises (no silent eager fallback). On CPU tensors (tests, CPU smoke runs) the plain
-PyTorch formulation is used.
+On a GPU the HIP kernels are mandatory for the types and sizes that an operator's docstring names: if
+the in-tree extension is missing or broken the first call raises (no silent eager fallback). Other types
+on a GPU (float64; float32 in cross_attention) and CPU tensors (tests, CPU smoke runs) take the plain
+PyTorch formulation. The kernels have first derivatives in reverse mode; rotary, dropout and cross
+attention refuse second and forward-mode ones on a GPU.
 """
 
 from __future__ import annotations
